@@ -53,7 +53,10 @@ enum rocshmem_amd_dtype {
   ROCSHMEM_AMD_CHAR = 10,
   ROCSHMEM_AMD_SCHAR = 11,
   ROCSHMEM_AMD_UCHAR = 12,
-  ROCSHMEM_AMD_USHORT = 13
+  ROCSHMEM_AMD_USHORT = 13,
+  /* the key-value cache only: IEEE half, and OCP 8-bit float e4m3 ("fn") */
+  ROCSHMEM_AMD_HALF = 14,
+  ROCSHMEM_AMD_E4M3 = 15
 };
 
 /* Reduction operators: values of ROCSHMEM_OP (rocshmem_common.hpp:40-49). */
@@ -658,6 +661,130 @@ int rocshmem_amd_poll_until(int dtype, void *ivar, int cmp, const void *value, u
  * pe_out / npes_out (host arrays), then destroys them all. */
 int rocshmem_amd_ctx_cycle(rocshmem_amd_team_t team, int n_wgs, int wg_size, int per_wg,
                            int *status_out, int *pe_out, int *npes_out);
+
+/* ============== key-value cache on the symmetric heap ====================== */
+
+/* A model that answers with a cache keeps, for every token it has seen, one key
+ * row and one value row per cache head.  Here that cache is a symmetric object
+ * of pages spread over the PEs: a token's rows are put to whichever PE owns its
+ * page, and read from there.  No reference counterpart.
+ *
+ * Pages hold page_tokens tokens each (a multiple of 16) and are numbered over
+ * all PEs: PE p owns pages p * pages_per_pe up to (p + 1) * pages_per_pe, one after
+ * the other at `pages`.  Slot s of the cache is token s mod page_tokens of page
+ * s / page_tokens.  A page is one contiguous block of rocshmem_amd_kv_page_bytes:
+ * keys [kv_heads][page_tokens][head_dim], then values alike, then for E4M3 one
+ * scale byte per key row and per value row ([kv_heads][page_tokens] each),
+ * padded to 128 bytes; moving it to another PE is one putmem.
+ *
+ * dtype: BF16, HALF, or E4M3 — rows narrowed to 8 bits with one power-of-two
+ * scale per row.  A row x is stored as round-to-nearest-even e4m3 of x / 2^e
+ * with e the smallest integer, from -126 up, for which the row's largest finite
+ * magnitude is at most 448 * 2^e, and the scale byte e + 127.  Dividing by a power
+ * of two is exact, so a code depends on nothing but the row and the format.
+ * Infinities and NaN are stored as NaN.
+ *
+ * All calls below act for PE my_pe, take `pages` (like every symmetric address)
+ * as my_pe's, only enqueue on `stream`, allocate nothing and may be captured
+ * into a graph; they run on the device the heap is on, which must be the
+ * current one.  As with putmem, rows put to another PE may be read there after
+ * a barrier (or stream order, where all PEs share the stream).  Slots, page
+ * numbers and lengths are read by the kernels; what is out of range is left
+ * out, never followed, and counted (rocshmem_amd_kv_refused). */
+typedef struct rocshmem_amd_kv_cache {
+  void *pages;      /* symmetric: pages_per_pe * page_bytes per PE, 16-byte aligned */
+  int dtype;        /* ROCSHMEM_AMD_BF16, _HALF or _E4M3 */
+  int pages_per_pe;
+  int page_tokens;  /* a multiple of 16, at most 65536 */
+  int kv_heads;     /* at most 4096 */
+  int head_dim;     /* a multiple of 16, at most 256 */
+} rocshmem_amd_kv_cache_t;
+
+/* Bytes of one page; 0 if there is no such cache. */
+size_t rocshmem_amd_kv_page_bytes(int dtype, int page_tokens, int kv_heads, int head_dim);
+/* Where slot `slot`'s row of cache head `head` lies (value != 0: its value row,
+ * else its key row): the PE that owns it, its offset from `pages` on that PE,
+ * and (E4M3; else the row's own offset) the offset of its scale byte.  The
+ * arithmetic of the kernels, usable without a GPU; cache->pages is not looked
+ * at.  -1 if the slot or head does not exist among npes PEs. */
+int rocshmem_amd_kv_row(const rocshmem_amd_kv_cache_t *cache, int npes, int64_t slot, int head,
+                        int value, int *pe_out, uint64_t *offset_out, uint64_t *scale_offset_out);
+
+/* Puts n_tokens tokens' rows into their slots.  k, v: device memory of `dtype`
+ * (BF16, HALF or FLOAT), token t's rows at k + t * k_row elements (v_row for v),
+ * its heads one after the other; slots: n_tokens device integers.  A slot of -1
+ * leaves its token out (padding).  Slots that are named twice in one call end
+ * up with a mixture of the rows given for them; everything else is as if the
+ * tokens had been put one after the other. */
+int rocshmem_amd_kv_put(const rocshmem_amd_kv_cache_t *cache, int dtype, const void *k, size_t k_row,
+                        const void *v, size_t v_row, const int64_t *slots, size_t n_tokens, int my_pe,
+                        rocshmem_amd_stream_t stream);
+/* Reads n_tokens tokens' rows back, widened or rounded to `dtype` (a value
+ * beyond its range becomes an infinity; a row of E4M3 may hold such a value
+ * where its largest one was rounded up).  The rows of a token whose slot is
+ * -1 or out of range are left as they were.  k_row and v_row are at least
+ * kv_heads * head_dim. */
+int rocshmem_amd_kv_get(const rocshmem_amd_kv_cache_t *cache, int dtype, void *k, size_t k_row, void *v,
+                        size_t v_row, const int64_t *slots, size_t n_tokens, int my_pe,
+                        rocshmem_amd_stream_t stream);
+
+/* Attention of one new token per sequence over its cached tokens.
+ *
+ * Sequence b has lengths[b] tokens; token i of it is token i mod page_tokens of
+ * page page_table[b * table_row + i / page_tokens].  With window > 0 only the last
+ * `window` tokens take part.  Query head h of q_heads (a multiple of kv_heads)
+ * looks at cache head h / (q_heads / kv_heads):
+ *
+ *   s_i = scale * <q, k_i>, softcap > 0: s_i = softcap * tanh(s_i / softcap)
+ *   out = sum_i exp(s_i) v_i / sum_i exp(s_i),   lse = log sum_i exp(s_i)
+ *
+ * with the sums over the tokens that take part; where none does, out is 0 and
+ * lse -infinity.  Scores, statistics and sums are held in 32 bits.
+ * pages_from: ROCSHMEM_AMD_KV_ALL_PAGES, or ROCSHMEM_AMD_KV_OWN_PAGES — only the
+ * tokens whose page my_pe owns take part, and rocshmem_amd_kv_join of the PEs'
+ * results is the attention over all of them.
+ *
+ * q: n_seqs x q_heads x head_dim of `dtype` (the cache's, or BF16 or HALF for an
+ * E4M3 cache), sequence b's at q + b * q_row elements.  out: the same shape in
+ * out_dtype (`dtype`, or FLOAT for partial results), rows out_row elements
+ * apart (at least q_heads * head_dim).  lse: n_seqs x q_heads floats, or NULL.
+ * A length above max_len, or above what table_row pages hold, counts as that
+ * (and is counted as refused); a negative one as 0 (the same).
+ * workspace: device memory of at least rocshmem_amd_kv_attend_bytes bytes,
+ * 16-byte aligned, whose content does not matter; calls that may overlap in
+ * time need one each. */
+enum rocshmem_amd_kv_pages_from { ROCSHMEM_AMD_KV_ALL_PAGES = 0, ROCSHMEM_AMD_KV_OWN_PAGES = 1 };
+size_t rocshmem_amd_kv_attend_bytes(const rocshmem_amd_kv_cache_t *cache, int n_seqs, int q_heads,
+                                    int max_len);
+int rocshmem_amd_kv_attend(const rocshmem_amd_kv_cache_t *cache, int dtype, const void *q, size_t q_row,
+                           int q_heads, int out_dtype, void *out, size_t out_row, float *lse,
+                           const int32_t *page_table, size_t table_row, const int32_t *lengths,
+                           int n_seqs, int max_len, int window, float scale, float softcap,
+                           int pages_from, void *workspace, size_t workspace_bytes, int my_pe,
+                           rocshmem_amd_stream_t stream);
+
+/* Joins what the PEs of the active set reached over their own shares of the
+ * tokens: member i's partial results o_i (n_rows x head_dim of `dtype`: BF16,
+ * HALF or FLOAT) with lse_i (n_rows floats), both symmetric and given as my_pe's
+ * addresses, are read from every member's slice and
+ *
+ *   out = sum_i exp(lse_i) o_i / sum_i exp(lse_i),   lse = log sum_i exp(lse_i)
+ *
+ * goes to my_pe's out (out_dtype: BF16, HALF or FLOAT) and lse (may be NULL).  A
+ * member whose lse_i is -infinity takes no part, whatever its o_i holds; with
+ * none left out is 0 and lse -infinity.  One-sided, like a get: call it once
+ * the members' results are complete.  The members are folded in ascending
+ * order.  head_dim: a multiple of 8; partial 16-byte aligned. */
+int rocshmem_amd_kv_join(int dtype, const void *partial, const float *partial_lse, size_t n_rows,
+                         int head_dim, int out_dtype, void *out, float *lse, int PE_start,
+                         int logPE_stride, int PE_size, int my_pe, rocshmem_amd_stream_t stream);
+
+/* How many slots, page numbers and lengths the calls above have left out or cut
+ * because they were out of range, since the count was last cleared (clear != 0
+ * clears it).  A slot of -1 is padding and not counted; an entry of the page
+ * table counts once a call, if any of its tokens would have taken part.  Call
+ * it after waiting for the kernels.  -1 before rocshmem_init. */
+int64_t rocshmem_amd_kv_refused(int clear);
 
 #ifdef __cplusplus
 }

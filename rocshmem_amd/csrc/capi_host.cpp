@@ -63,6 +63,10 @@ int64_t rocshmem_amd_waits_given_up(int clear) {
   if (!rt().live) return -1;
   return static_cast<int64_t>(rt().waits_given_up(clear != 0));
 }
+int64_t rocshmem_amd_kv_refused(int clear) {
+  if (!rt().live) return -1;
+  return static_cast<int64_t>(rt().kv_refused(clear != 0));
+}
 int rocshmem_amd_set_coalesce_puts(int on) {
   if (!rt().live) return -1;
   const int before = rt().state.coalesce_puts;

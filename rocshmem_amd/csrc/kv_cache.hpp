@@ -1,0 +1,131 @@
+// The paged key-value cache on the symmetric heap: where a token's rows lie,
+// and the checks its entry points share.  The arithmetic is plain C++ used by
+// host and device code alike.
+//
+// Pages of a fixed number of tokens are numbered over all PEs: PE p holds pages
+// p * pages_per_pe up to (p + 1) * pages_per_pe, one after the other in one
+// symmetric object.  A page is one contiguous block, so that moving a page to
+// another PE is one putmem:
+//
+//   keys   [kv_heads][page_tokens][head_dim]
+//   values [kv_heads][page_tokens][head_dim]
+//   e4m3 only: key scales [kv_heads][page_tokens], value scales, one byte each
+//   padding to a multiple of 128 bytes
+//
+// Head-major within the page: attention reads one head's tokens of a page as
+// one run of page_tokens * head_dim elements.
+#ifndef ROCSHMEM_AMD_KV_CACHE_HPP_
+#define ROCSHMEM_AMD_KV_CACHE_HPP_
+
+#include <hip/hip_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+#include "rocshmem_amd.h"
+
+namespace rocshmem {
+namespace kv {
+
+constexpr int kTokenUnit = 16;  // page_tokens and head_dim are multiples of it
+constexpr int kMaxHeadDim = 256;
+
+// n / d for 0 <= n < 2^31 as a multiplication: mul = floor(2^(31+l) / d) + 1 with
+// l = ceil(log2 d), so that 0 < mul * d - 2^(31+l) <= 2^l and the quotient is
+// exact; mul fits in 32 bits because d > 2^(l-1).
+struct Divisor {
+  uint32_t d, mul, shift;
+};
+__host__ __device__ inline Divisor make_divisor(uint32_t d) {
+  uint32_t l = 0;
+  while ((uint64_t{1} << l) < d) ++l;
+  return Divisor{d, static_cast<uint32_t>((uint64_t{1} << (31 + l)) / d + 1), 31 + l};
+}
+__host__ __device__ inline uint32_t quotient(uint32_t n, const Divisor &by) {
+  return static_cast<uint32_t>((static_cast<uint64_t>(n) * by.mul) >> by.shift);
+}
+
+inline int element_bytes(int dtype) {
+  switch (dtype) {
+    case ROCSHMEM_AMD_FLOAT: return 4;
+    case ROCSHMEM_AMD_BF16:
+    case ROCSHMEM_AMD_HALF: return 2;
+    case ROCSHMEM_AMD_E4M3: return 1;
+    default: return 0;
+  }
+}
+
+struct Layout {
+  char *pages;          // this PE's copy of the symmetric object
+  uint64_t page_bytes;
+  uint64_t value_offset;                       // from the start of a page
+  uint64_t key_scale_offset, value_scale_offset;
+  uint32_t row_bytes;                          // one token's row of one head
+  uint32_t page_tokens, kv_heads, head_dim;
+  uint32_t pages_per_pe, n_pages;              // n_pages: over all PEs
+  Divisor by_page_units;                       // page_tokens / 16
+  Divisor by_pages_per_pe;
+};
+
+struct Place {
+  uint32_t page, at;  // page over all PEs, token within it
+};
+__host__ __device__ inline bool slot_in_range(const Layout &c, int64_t slot) {
+  return slot >= 0 && slot < static_cast<int64_t>(c.n_pages) * c.page_tokens;
+}
+// Slots are divided in units of 16 tokens, so that every quotient is one of
+// 31-bit numbers (fill_layout refuses a cache with more units).
+__host__ __device__ inline Place place_of(const Layout &c, int64_t slot) {
+  Place p;
+  p.page = quotient(static_cast<uint32_t>(slot >> 4), c.by_page_units);
+  p.at = static_cast<uint32_t>(slot - static_cast<int64_t>(p.page) * c.page_tokens);
+  return p;
+}
+__host__ __device__ inline uint32_t owner_of(const Layout &c, uint32_t page) {
+  return quotient(page, c.by_pages_per_pe);
+}
+// Offset of a page from the start of its owner's copy.
+__host__ __device__ inline uint64_t page_offset(const Layout &c, uint32_t page, uint32_t owner) {
+  return static_cast<uint64_t>(page - owner * c.pages_per_pe) * c.page_bytes;
+}
+// Offset within a page of token `at`'s row of head `head`; its scale byte.
+__host__ __device__ inline uint64_t row_offset(const Layout &c, uint32_t head, uint32_t at, bool value) {
+  return (value ? c.value_offset : 0) +
+         static_cast<uint64_t>(head * c.page_tokens + at) * c.row_bytes;
+}
+__host__ __device__ inline uint64_t scale_offset(const Layout &c, uint32_t head, uint32_t at, bool value) {
+  return (value ? c.value_scale_offset : c.key_scale_offset) + head * c.page_tokens + at;
+}
+
+// Fills in everything but `pages`; false for a cache that is not supported.
+inline bool fill_layout(int dtype, int page_tokens, int kv_heads, int head_dim, int64_t pages_per_pe,
+                        int npes, Layout *out) {
+  const int es = dtype == ROCSHMEM_AMD_FLOAT ? 0 : element_bytes(dtype);
+  if (!es || page_tokens < kTokenUnit || page_tokens % kTokenUnit || page_tokens > 65536) return false;
+  if (head_dim < kTokenUnit || head_dim % kTokenUnit || head_dim > kMaxHeadDim) return false;
+  if (kv_heads < 1 || kv_heads > 4096 || pages_per_pe < 1 || npes < 1) return false;
+  const int64_t units = page_tokens / kTokenUnit;
+  if (pages_per_pe > INT32_MAX || pages_per_pe * npes > INT32_MAX / units) return false;
+  Layout c{};
+  c.row_bytes = static_cast<uint32_t>(head_dim * es);
+  c.page_tokens = static_cast<uint32_t>(page_tokens);
+  c.kv_heads = static_cast<uint32_t>(kv_heads);
+  c.head_dim = static_cast<uint32_t>(head_dim);
+  const uint64_t rows = static_cast<uint64_t>(kv_heads) * page_tokens;  // < 2^28
+  c.value_offset = rows * c.row_bytes;
+  c.key_scale_offset = 2 * c.value_offset;
+  c.value_scale_offset = c.key_scale_offset + rows;
+  const uint64_t used = c.key_scale_offset + (dtype == ROCSHMEM_AMD_E4M3 ? 2 * rows : 0);
+  c.page_bytes = (used + 127) / 128 * 128;
+  c.pages_per_pe = static_cast<uint32_t>(pages_per_pe);
+  c.n_pages = static_cast<uint32_t>(pages_per_pe * npes);
+  c.by_page_units = make_divisor(static_cast<uint32_t>(units));
+  c.by_pages_per_pe = make_divisor(c.pages_per_pe);
+  *out = c;
+  return true;
+}
+
+}  // namespace kv
+}  // namespace rocshmem
+
+#endif  // ROCSHMEM_AMD_KV_CACHE_HPP_

@@ -688,6 +688,9 @@ int Runtime::init(int want_npes, size_t want_heap) {
   RT_CHECK_HIP(hipMalloc(reinterpret_cast<void **>(&d_gave_up), sizeof(unsigned long long)));
   RT_CHECK_HIP(hipMemset(d_gave_up, 0, sizeof(unsigned long long)));
   state.gave_up = d_gave_up;
+  RT_CHECK_HIP(hipGetDevice(&device));
+  RT_CHECK_HIP(hipMalloc(reinterpret_cast<void **>(&d_kv_refused), sizeof(unsigned long long)));
+  RT_CHECK_HIP(hipMemset(d_kv_refused, 0, sizeof(unsigned long long)));
   live = true;
   push_state();
   ROCSHMEM_TEAM_WORLD = team_handle(0, acting_pe);
@@ -711,6 +714,8 @@ void Runtime::finalize() {
   d_queue_table = nullptr;
   RT_CHECK_HIP(hipFree(d_gave_up));
   d_gave_up = nullptr;
+  RT_CHECK_HIP(hipFree(d_kv_refused));
+  d_kv_refused = nullptr;
   RT_CHECK_HIP(hipHostFree(h_bind_problem));
   h_bind_problem = nullptr;
   RT_CHECK_HIP(hipFree(d_pools));
@@ -898,6 +903,14 @@ uint64_t Runtime::waits_given_up(bool clear) {
   unsigned long long n = 0;
   RT_CHECK_HIP(hipMemcpy(&n, d_gave_up, sizeof(n), hipMemcpyDeviceToHost));
   if (clear && n) RT_CHECK_HIP(hipMemset(d_gave_up, 0, sizeof(n)));
+  return n;
+}
+
+uint64_t Runtime::kv_refused(bool clear) {
+  require_live("rocshmem_amd_kv_refused");
+  unsigned long long n = 0;
+  RT_CHECK_HIP(hipMemcpy(&n, d_kv_refused, sizeof(n), hipMemcpyDeviceToHost));
+  if (clear && n) RT_CHECK_HIP(hipMemset(d_kv_refused, 0, sizeof(n)));
   return n;
 }
 

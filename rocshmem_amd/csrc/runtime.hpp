@@ -24,6 +24,7 @@ struct Runtime {
   int acting_pe = 0;  // PE the host acts as outside PE threads (rocshmem_emu_set_pe)
   // PE the calling thread acts as.
   int me() const { return tl_pe >= 0 ? tl_pe : acting_pe; }
+  int device = 0;  // HIP device the heap is on
   int max_ctxs = 0;
   int max_teams = 0;
   int num_user_teams = 0;
@@ -53,6 +54,7 @@ struct Runtime {
   detail::CtxPool *d_pools = nullptr;      // [npes]
   detail::QueueBinding *d_queue_table = nullptr;  // [kQueueTableSize]
   unsigned long long *d_gave_up = nullptr;  // waits and barriers that ran into the spin limit
+  unsigned long long *d_kv_refused = nullptr;  // slots, pages and lengths the cache's kernels left out
   int *h_bind_problem = nullptr;  // pinned, [kQueueTableSize]: what each stream binding reported
   std::vector<detail::Team> h_teams;       // host mirror of d_teams
   std::vector<bool> team_slot_used;
@@ -93,6 +95,7 @@ struct Runtime {
   void set_coalesce_puts(int on);
   void set_spin_limit(uint64_t polls);
   uint64_t waits_given_up(bool clear);
+  uint64_t kv_refused(bool clear);
 
   // Context handle of PE `pe` bound to its member object of team slot `slot`.
   rocshmem_ctx_t default_ctx_handle(int pe, int slot = 0) const {

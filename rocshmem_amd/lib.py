@@ -8,7 +8,7 @@ LIB_PATH = os.path.join(_HERE, "lib", "librocshmem_amd.so")
 
 # Enumerations of include/rocshmem_amd.h.
 (SHORT, INT, LONG, LONGLONG, FLOAT, DOUBLE, BF16, UINT, ULONG, ULONGLONG, CHAR, SCHAR, UCHAR,
- USHORT) = range(14)
+ USHORT, HALF, E4M3) = range(16)
 SUM, MAX, MIN, PROD, AND, OR, XOR = range(7)
 THREAD, WAVE, WG = range(3)
 PUT, GET, PUT_NBI, GET_NBI = range(4)
@@ -19,9 +19,20 @@ TEST, WAIT_UNTIL, WAIT_UNTIL_ANY, WAIT_UNTIL_ALL, WAIT_UNTIL_SOME = range(5)
 BARRIER_ALL, SYNC_ALL, TEAM_SYNC = range(3)
 CMP_EQ, CMP_NE, CMP_GT, CMP_GE, CMP_LT, CMP_LE = range(6)
 SIGNAL_SET, SIGNAL_ADD = range(2)
+KV_ALL_PAGES, KV_OWN_PAGES = range(2)
 SIZE_MAX = (1 << 64) - 1
 
 _vp, _sz, _i, _u32, _u64 = C.c_void_p, C.c_size_t, C.c_int, C.c_uint32, C.c_uint64
+
+
+class KvCache(C.Structure):
+    """``rocshmem_amd_kv_cache_t``: a paged key-value cache on the symmetric heap."""
+
+    _fields_ = [("pages", _vp), ("dtype", _i), ("pages_per_pe", _i), ("page_tokens", _i), ("kv_heads", _i),
+                ("head_dim", _i)]
+
+
+_kv = C.POINTER(KvCache)
 
 # name -> (restype, argtypes); every symbol the header declares.
 SIGNATURES = {
@@ -131,6 +142,15 @@ SIGNATURES = {
     "rocshmem_amd_wait_test_woken": (_i, [_i, _i, _vp, _sz, _vp, _i, _vp, _sz, _vp, _u64,
                                           C.POINTER(_sz), _vp]),
     "rocshmem_amd_poll_until": (_i, [_i, _vp, _i, _vp, _u64, _vp, _vp]),
+    "rocshmem_amd_kv_page_bytes": (_sz, [_i, _i, _i, _i]),
+    "rocshmem_amd_kv_row": (_i, [_kv, _i, C.c_int64, _i, _i, C.POINTER(_i), C.POINTER(_u64), C.POINTER(_u64)]),
+    "rocshmem_amd_kv_put": (_i, [_kv, _i, _vp, _sz, _vp, _sz, _vp, _sz, _i, _vp]),
+    "rocshmem_amd_kv_get": (_i, [_kv, _i, _vp, _sz, _vp, _sz, _vp, _sz, _i, _vp]),
+    "rocshmem_amd_kv_attend_bytes": (_sz, [_kv, _i, _i, _i]),
+    "rocshmem_amd_kv_attend": (_i, [_kv, _i, _vp, _sz, _i, _i, _vp, _sz, _vp, _vp, _sz, _vp, _i, _i, _i,
+                                    C.c_float, C.c_float, _i, _vp, _sz, _i, _vp]),
+    "rocshmem_amd_kv_join": (_i, [_i, _vp, _vp, _sz, _i, _i, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "rocshmem_amd_kv_refused": (C.c_int64, [_i]),
     "rocshmem_amd_ctx_cycle": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp]),
 }
 
