@@ -1,116 +1,111 @@
 // Attention of one new token per sequence over the paged key-value cache.
-#include "kv_device.hpp"
+#include "kv_attend.hpp"
 
 namespace rocshmem {
 namespace kv {
 
-struct AttendArgs {
-  Layout cache;
-  const detail::Context *ctx;
-  unsigned long long *refused;
-  const char *q;
-  char *out;
-  float *lse;
-  const int32_t *page_table;
-  const int32_t *lengths;
-  uint64_t q_row, out_row;  // elements between sequences
-  uint64_t table_row;
-  int q_heads, group;       // query heads, and how many share a cache head
-  int max_len, window, my_pe;
-  bool own_pages;
-  float scale, softcap;
-};
+// A call is cut so that there are about this many work-groups (six for each of
+// 256 CUs), each with at least one step for every wavefront.
+constexpr int64_t kWantedWorkGroups = 1536;
+constexpr int64_t kMaxSplits = 4096;
 
-// The tokens of sequence b that take part: [first, end).
-struct Span {
-  int first, end;
-};
-__device__ __forceinline__ Span span_of(const AttendArgs &a, int b, bool counts) {
-  const int len = a.lengths[b];
-  int end = len < 0 ? 0 : len < a.max_len ? len : a.max_len;
-  const uint64_t held = a.table_row * a.cache.page_tokens;
-  if (static_cast<uint64_t>(end) > held) end = static_cast<int>(held);
-  if (end != len && counts) count_refused(a.refused);
-  return Span{a.window > 0 && end > a.window ? end - a.window : 0, end};
-}
-
-// One wavefront per sequence and query head.  64 tokens at a time, a lane for
-// each: the score, the running maximum and sum over the wavefront; then the
-// values token by token with the lanes along the row.
-template <int kIn, int kCache, int kOut>
-__global__ __launch_bounds__(64) void attend_kernel(AttendArgs a) {
-  const int b = blockIdx.y, h = blockIdx.x, lane = threadIdx.x;
-  const uint32_t head = static_cast<uint32_t>(h / a.group), d = a.cache.head_dim;
-  const Span span = span_of(a, b, h == 0 && lane == 0);
-  const char *q = a.q + (b * a.q_row + h * d) * Eight<kIn>::kBytes;
-  float top = -INFINITY, total = 0.f, acc[8] = {};
-  for (int t0 = span.first; t0 < span.end; t0 += 64) {
-    const int t = t0 + lane;
-    const char *page = nullptr;
-    uint32_t at = 0;
-    float s = -INFINITY;
-    if (t < span.end) {
-      const uint32_t index = quotient(static_cast<uint32_t>(t) >> 4, a.cache.by_page_units);
-      at = t - index * a.cache.page_tokens;
-      const uint32_t number = static_cast<uint32_t>(a.page_table[b * a.table_row + index]);
-      if (number >= a.cache.n_pages) {
-        if (h == 0 && (at == 0 || t == span.first)) count_refused(a.refused);
-      } else {
-        const uint32_t pe = owner_of(a.cache, number);
-        if (!a.own_pages || static_cast<int>(pe) == a.my_pe)
-          page = detail::remote_addr(a.ctx, a.cache.pages, static_cast<int>(pe)) +
-                 page_offset(a.cache, number, pe);
-      }
-    }
-    if (page) {
-      const char *k = page + row_offset(a.cache, head, at, false);
-      float dot = 0.f;
-      for (uint32_t e = 0; e < d; e += 8) {
-        float x[8], y[8];
-        Eight<kIn>::widen(Eight<kIn>::load(q + e * Eight<kIn>::kBytes), x);
-        Eight<kCache>::widen(Eight<kCache>::load(k + e * Eight<kCache>::kBytes), y);
-        for (int i = 0; i < 8; ++i) dot += x[i] * y[i];
-      }
-      if (kCache == ROCSHMEM_AMD_E4M3)
-        dot *= two_to(static_cast<unsigned char>(page[scale_offset(a.cache, head, at, false)]));
-      s = dot * a.scale;
-      if (a.softcap > 0.f) s = a.softcap * tanhf(s / a.softcap);
-    }
-    float tile_top = s;
-    for (int hop = 32; hop; hop /= 2) tile_top = fmaxf(tile_top, __shfl_xor(tile_top, hop));
-    const float next = fmaxf(top, tile_top), from = next == -INFINITY ? 0.f : next;
-    const float p = expf(s - from), keep = expf(top - from);
-    float sum = p;
-    for (int hop = 32; hop; hop /= 2) sum += __shfl_xor(sum, hop);
-    total = total * keep + sum;
-    for (int i = 0; i < 8; ++i) acc[i] *= keep;
-    top = next;
-    const int n = span.end - t0 < 64 ? span.end - t0 : 64;
-    for (int j = 0; j < n; ++j) {
-      const char *from_page = reinterpret_cast<const char *>(
-          __shfl(static_cast<unsigned long long>(reinterpret_cast<uintptr_t>(page)), j));
-      const uint32_t from_at = __shfl(at, j);
-      float w = __shfl(p, j);
-      if (!from_page || lane * 8u >= d) continue;
-      float y[8];
-      Eight<kCache>::widen(
-          Eight<kCache>::load(from_page + row_offset(a.cache, head, from_at, true) + lane * 8 * Eight<kCache>::kBytes), y);
-      if (kCache == ROCSHMEM_AMD_E4M3)
-        w *= two_to(static_cast<unsigned char>(from_page[scale_offset(a.cache, head, from_at, true)]));
-      for (int i = 0; i < 8; ++i) acc[i] += w * y[i];
-    }
+// Joins a sequence's splits: out = sum_i 2^(t_i - t) o_i / sum_i 2^(t_i - t) l_i over the
+// splits that have tokens, t the largest t_i.  One work-group per sequence and
+// query head; 64 lanes along the row, the splits dealt out to the four wavefronts.
+__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
+  const int b = blockIdx.y, h = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Span span = span_of(a, b, false);
+  const int units = span.end_unit() - span.first_unit();
+  if (units <= a.split_units) return;  // its only split has written the result
+  const int n = (units + a.split_units - 1) / a.split_units;
+  const uint64_t row = static_cast<uint64_t>(b) * a.q_heads + h;
+  const F2 *stat = a.part_stat + row * a.splits;
+  const uint32_t d = a.cache.head_dim;
+  __shared__ float sh_top[4], sh_total[4];
+  __shared__ F4 sh_out[4][64];
+  float top = -INFINITY;
+  for (int i = threadIdx.x; i < n; i += 256) top = fmaxf(top, stat[i].x);
+  for (int hop = 32; hop; hop /= 2) top = fmaxf(top, __shfl_xor(top, hop));
+  if (lane == 0) sh_top[wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(sh_top[0], sh_top[1]), fmaxf(sh_top[2], sh_top[3]));
+  const float from = top == -INFINITY ? 0.f : top;
+  float total = 0.f;
+  F4 x{0.f, 0.f, 0.f, 0.f};
+  for (int i = wave; i < n; i += 4) {
+    const F2 s = stat[i];
+    const float w = __builtin_amdgcn_exp2f(s.x - from);
+    total += w * s.y;
+    if (lane * 4u < d) x += w * *reinterpret_cast<const F4 *>(a.part + (row * a.splits + i) * d + lane * 4);
   }
+  sh_out[wave][lane] = x;
+  if (lane == 0) sh_total[wave] = total;
+  __syncthreads();
+  total = sh_total[0] + sh_total[1] + sh_total[2] + sh_total[3];
   const float inv = total == 0.f ? 0.f : 1.f / total;
-  for (int i = 0; i < 8; ++i) acc[i] *= inv;
-  if (lane * 8u < d)
-    Eight<kOut>::store(a.out + (b * a.out_row + h * d + lane * 8) * Eight<kOut>::kBytes, Eight<kOut>::round(acc));
-  if (a.lse && lane == 0) a.lse[static_cast<uint64_t>(b) * a.q_heads + h] = top + logf(total);
+  if (threadIdx.x * 8 < d) {
+    float y[8] = {};
+    for (int w = 0; w < 4; ++w)
+      for (int e = 0; e < 8; ++e) y[e] += sh_out[w][threadIdx.x * 2 + e / 4][e % 4];
+    for (int e = 0; e < 8; ++e) y[e] *= inv;
+    store_out(a, b, h, threadIdx.x * 8, y);
+  }
+  if (a.lse && threadIdx.x == 0) a.lse[row] = (top + __builtin_amdgcn_logf(total)) * kLn2;
 }
 
-template <int kIn, int kCache, int kOut>
+// How a call is cut: tokens of a split (in units of 16) and how many splits the
+// longest sequence can have.
+struct Cut {
+  int units, splits;
+};
+static Cut cut_of(int64_t work_groups_per_split, int64_t max_tokens) {
+  const int64_t units = (max_tokens + 15) / 16 + 1;  // a window may start inside a unit
+  const int64_t wanted = (kWantedWorkGroups + work_groups_per_split - 1) / work_groups_per_split;
+  int64_t each = (units + wanted - 1) / wanted;
+  each = (each + 7) / 8 * 8;  // a step of every wavefront
+  if (each > 64) each = 64;
+  while ((units + each - 1) / each > kMaxSplits) each *= 2;
+  return Cut{static_cast<int>(each), static_cast<int>((units + each - 1) / each)};
+}
+static int columns_of(int group, int head_dim) {  // tiles of 16 query heads that one work-group takes
+  const int tiles = (group + 15) / 16;
+  const int most = head_dim > 128 ? 2 : 4;
+  return tiles < most ? tiles : most;
+}
+static size_t part_bytes(size_t rows, size_t splits, size_t head_dim) {
+  return splits > 1 ? rows * splits * (head_dim + 2) * sizeof(float) : 0;
+}
+
+template <int kQ, int kC, int kDim>
+static void launch_columns(const AttendArgs &a, int columns, dim3 grid, hipStream_t s) {
+  const dim3 block(64 * kAttendWaves);
+  switch (columns) {
+    case 1: hipLaunchKernelGGL((attend_kernel<kQ, kC, kDim, 1>), grid, block, 0, s, a); return;
+    case 2: hipLaunchKernelGGL((attend_kernel<kQ, kC, kDim, 2>), grid, block, 0, s, a); return;
+    default: break;
+  }
+  if constexpr (kDim <= 128) {
+    if (columns == 3)
+      hipLaunchKernelGGL((attend_kernel<kQ, kC, kDim, 3>), grid, block, 0, s, a);
+    else
+      hipLaunchKernelGGL((attend_kernel<kQ, kC, kDim, 4>), grid, block, 0, s, a);
+  }
+}
+template <int kQ, int kC>
 static void launch_attend(const AttendArgs &a, int n_seqs, hipStream_t s) {
-  hipLaunchKernelGGL((attend_kernel<kIn, kCache, kOut>), dim3(a.q_heads, n_seqs), dim3(64), 0, s, a);
+  const int columns = columns_of(a.group, static_cast<int>(a.cache.head_dim));
+  const dim3 grid(a.cache.kv_heads * a.tiles, n_seqs, a.splits);
+  if (a.cache.head_dim <= 64)
+    launch_columns<kQ, kC, 64>(a, columns, grid, s);
+  else if (a.cache.head_dim <= 128)
+    launch_columns<kQ, kC, 128>(a, columns, grid, s);
+  else
+    launch_columns<kQ, kC, 256>(a, columns, grid, s);
   DRV_CHECK_HIP(hipGetLastError());
+  if (a.splits > 1) {
+    hipLaunchKernelGGL(attend_join_kernel, dim3(a.q_heads, n_seqs), dim3(256), 0, s, a);
+    DRV_CHECK_HIP(hipGetLastError());
+  }
 }
 
 }  // namespace kv
@@ -121,7 +116,15 @@ using namespace rocshmem::kv;
 
 extern "C" {
 
-size_t rocshmem_amd_kv_attend_bytes(const rocshmem_amd_kv_cache_t *, int, int, int) { return 0; }
+size_t rocshmem_amd_kv_attend_bytes(const rocshmem_amd_kv_cache_t *cache, int n_seqs, int q_heads, int max_len) {
+  Layout c;
+  if (!cache || !fill_layout(cache->dtype, cache->page_tokens, cache->kv_heads, cache->head_dim, 1, 1, &c)) return 0;
+  if (n_seqs < 1 || n_seqs > 65535 || max_len < 1 || q_heads < 1 || q_heads > 65535 || q_heads % cache->kv_heads) return 0;
+  const int group = q_heads / cache->kv_heads, columns = columns_of(group, cache->head_dim);
+  const int64_t tiles = (group + 16 * columns - 1) / (16 * columns);
+  return part_bytes(static_cast<size_t>(n_seqs) * q_heads,
+                    cut_of(n_seqs * tiles * cache->kv_heads, max_len).splits, c.head_dim);
+}
 
 int rocshmem_amd_kv_attend(const rocshmem_amd_kv_cache_t *cache, int dtype, const void *q, size_t q_row,
                            int q_heads, int out_dtype, void *out, size_t out_row, float *lse,
@@ -152,8 +155,25 @@ int rocshmem_amd_kv_attend(const rocshmem_amd_kv_cache_t *cache, int dtype, cons
   if (!lengths || !aligned_to(lengths, 4) || !drv::local_ok(lengths, 4 * static_cast<size_t>(n_seqs))) return -1;
   if (!aligned_to(page_table, 4) || !drv::local_ok(page_table, table_bytes)) return -1;
   if (table_row > static_cast<size_t>(INT32_MAX)) return -1;
-  (void)workspace;
-  (void)workspace_bytes;
+  const size_t rows = static_cast<size_t>(n_seqs) * q_heads;
+  a.group = q_heads / cache->kv_heads;
+  const int columns = columns_of(a.group, cache->head_dim);
+  a.tiles = (a.group + 16 * columns - 1) / (16 * columns);
+  const int64_t per_split = static_cast<int64_t>(n_seqs) * cache->kv_heads * a.tiles;
+  const size_t needed = part_bytes(rows, cut_of(per_split, max_len).splits, a.cache.head_dim);
+  if (needed && (!workspace || !aligned_to(workspace, 16) || workspace_bytes < needed ||
+                 !drv::local_ok(workspace, workspace_bytes)))
+    return -1;
+  const Cut cut = cut_of(per_split, window > 0 && window < max_len ? window : max_len);
+  a.split_units = cut.units;
+  a.splits = cut.splits;
+  while (part_bytes(rows, a.splits, a.cache.head_dim) > needed) {  // a window is cut no finer than the whole
+    a.split_units *= 2;
+    a.splits = (a.splits + 1) / 2;
+  }
+  a.part = static_cast<float *>(workspace);
+  a.part_stat = reinterpret_cast<F2 *>(a.part + rows * a.splits * a.cache.head_dim);
+  a.out_dtype = out_dtype;
   a.ctx = reinterpret_cast<const detail::Context *>(runtime::rt().driver_ctx_handle(my_pe).ctx_opaque);
   a.refused = runtime::rt().d_kv_refused;
   a.q = static_cast<const char *>(q);
@@ -165,7 +185,6 @@ int rocshmem_amd_kv_attend(const rocshmem_amd_kv_cache_t *cache, int dtype, cons
   a.out_row = out_row;
   a.table_row = table_row;
   a.q_heads = q_heads;
-  a.group = q_heads / cache->kv_heads;
   a.max_len = max_len;
   a.window = window;
   a.my_pe = my_pe;
@@ -173,18 +192,14 @@ int rocshmem_amd_kv_attend(const rocshmem_amd_kv_cache_t *cache, int dtype, cons
   a.scale = scale;
   a.softcap = softcap;
   hipStream_t s = drv::as_stream(stream);
-  const auto to = [&](auto in) {
-    constexpr int kIn = decltype(in)::value;
-    const bool narrow = cache->dtype == ROCSHMEM_AMD_E4M3, wide = out_dtype == ROCSHMEM_AMD_FLOAT;
-    if (narrow && wide) launch_attend<kIn, ROCSHMEM_AMD_E4M3, ROCSHMEM_AMD_FLOAT>(a, n_seqs, s);
-    if (narrow && !wide) launch_attend<kIn, ROCSHMEM_AMD_E4M3, kIn>(a, n_seqs, s);
-    if (!narrow && wide) launch_attend<kIn, kIn, ROCSHMEM_AMD_FLOAT>(a, n_seqs, s);
-    if (!narrow && !wide) launch_attend<kIn, kIn, kIn>(a, n_seqs, s);
-  };
-  if (dtype == ROCSHMEM_AMD_BF16)
-    to(std::integral_constant<int, ROCSHMEM_AMD_BF16>{});
+  if (cache->dtype == ROCSHMEM_AMD_BF16)
+    launch_attend<ROCSHMEM_AMD_BF16, ROCSHMEM_AMD_BF16>(a, n_seqs, s);
+  else if (cache->dtype == ROCSHMEM_AMD_HALF)
+    launch_attend<ROCSHMEM_AMD_HALF, ROCSHMEM_AMD_HALF>(a, n_seqs, s);
+  else if (dtype == ROCSHMEM_AMD_BF16)
+    launch_attend<ROCSHMEM_AMD_BF16, ROCSHMEM_AMD_E4M3>(a, n_seqs, s);
   else
-    to(std::integral_constant<int, ROCSHMEM_AMD_HALF>{});
+    launch_attend<ROCSHMEM_AMD_HALF, ROCSHMEM_AMD_E4M3>(a, n_seqs, s);
   return 0;
 }
 

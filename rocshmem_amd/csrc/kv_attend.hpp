@@ -1,0 +1,529 @@
+// Attention of one new token per sequence over the paged key-value cache: the
+// kernel, and how a call's work is cut into work-groups.
+//
+//   s_t = scale <q, k_t>,  out = sum_t exp(s_t) v_t / sum_t exp(s_t)
+//
+// One pass over the tokens with a running maximum and sum.  The query heads that
+// share a cache head are the columns of matrix products, so keys and values are
+// read once for all of them, and nothing but the query, the running sums and
+// one step of keys and values is held, all of it in registers:
+//
+//   S^T (tokens x heads) = K Q^T,  O^T (dims x heads) += V^T P^T
+//
+// with v_mfma_f32_16x16x32.  A lane of the product S^T ends up with four
+// consecutive tokens of one head, and the product O^T wants eight tokens of one
+// head in a lane as its right operand; the order of a product's inner index is
+// free as long as both operands agree, so the eight are the lane's four of each
+// of two 16-token units, and P never leaves its lane.  V^T's lane then needs the
+// same eight tokens at one column; a lane loads a contiguous piece of each of its
+// eight tokens' rows (whole rows side by side across the lanes) and pairs up
+// tokens with byte permutes: columns are dealt out so that a lane's piece is one
+// element of each of the product's tiles.  No value goes through LDS on the way.
+#ifndef ROCSHMEM_AMD_KV_ATTEND_HPP_
+#define ROCSHMEM_AMD_KV_ATTEND_HPP_
+
+#include "kv_device.hpp"
+
+namespace rocshmem {
+namespace kv {
+
+struct AttendArgs {
+  Layout cache;
+  const detail::Context *ctx;
+  unsigned long long *refused;
+  const char *q;
+  char *out;
+  float *lse;
+  const int32_t *page_table;
+  const int32_t *lengths;
+  float *part;        // [sequence][query head][split][head_dim], not yet divided
+  F2 *part_stat;      // [sequence][query head][split]: exponent the sums are taken from, and sum
+  uint64_t q_row, out_row;  // elements between sequences
+  uint64_t table_row;
+  int q_heads, group, tiles;  // query heads; how many share a cache head; work-groups that share them out
+  int max_len, window, my_pe;
+  int split_units, splits;    // tokens of a split in units of 16, and how many at most
+  int out_dtype;
+  bool own_pages;
+  float scale, softcap;
+};
+
+// The tokens of a sequence that take part: [first, end).
+struct Span {
+  int first, end;
+  __device__ __forceinline__ int first_unit() const { return first >> 4; }
+  __device__ __forceinline__ int end_unit() const { return (end + 15) >> 4; }
+};
+__device__ __forceinline__ Span span_of(const AttendArgs &a, int b, bool counts) {
+  const int len = a.lengths[b];
+  int end = len < 0 ? 0 : len < a.max_len ? len : a.max_len;
+  const uint64_t held = a.table_row * a.cache.page_tokens;
+  if (static_cast<uint64_t>(end) > held) end = static_cast<int>(held);
+  if (end != len && counts) count_refused(a.refused);
+  return Span{a.window > 0 && end > a.window ? end - a.window : 0, end};
+}
+
+// Eight elements of a result row in the type that was asked for.
+__device__ __forceinline__ void store_out(const AttendArgs &a, int b, int h, int e, const float (&x)[8]) {
+  const uint64_t at = b * a.out_row + static_cast<uint64_t>(h) * a.cache.head_dim + e;
+  if (a.out_dtype == ROCSHMEM_AMD_FLOAT)
+    Eight<ROCSHMEM_AMD_FLOAT>::store(a.out + at * 4, Eight<ROCSHMEM_AMD_FLOAT>::round(x));
+  else if (a.out_dtype == ROCSHMEM_AMD_BF16)
+    Eight<ROCSHMEM_AMD_BF16>::store(a.out + at * 2, Eight<ROCSHMEM_AMD_BF16>::round(x));
+  else
+    Eight<ROCSHMEM_AMD_HALF>::store(a.out + at * 2, Eight<ROCSHMEM_AMD_HALF>::round(x));
+}
+
+typedef const __attribute__((address_space(1))) char *GlobalBytes;
+template <typename V>
+__device__ __forceinline__ V read_at(GlobalBytes from, uint32_t offset) {
+  return *(const __attribute__((address_space(1))) V *)(from + offset);  // NOLINT
+}
+
+constexpr int kAttendWaves = 4;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+// The matrix product of a type, and pairs of values rounded to it.
+template <int kType>
+struct Mma;
+template <>
+struct Mma<ROCSHMEM_AMD_BF16> {
+  using V = B8;
+  using E = __bf16;
+  __device__ __forceinline__ static F4 mul(V a, V b, F4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  template <bool kHigh>
+  __device__ __forceinline__ static unsigned from_e4m3(unsigned codes) {
+    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, kHigh));
+  }
+};
+template <>
+struct Mma<ROCSHMEM_AMD_HALF> {
+  using V = H8;
+  using E = _Float16;
+  __device__ __forceinline__ static F4 mul(V a, V b, F4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  template <bool kHigh>
+  __device__ __forceinline__ static unsigned from_e4m3(unsigned codes) {
+    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.0f, kHigh));
+  }
+};
+
+// The larger of the four lanes 16 apart that share a column, in all of them.
+__device__ __forceinline__ float max_of_column(float x) {
+  unsigned u = __float_as_uint(x);
+  auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  u = __float_as_uint(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+  r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_of_column(float x) {
+  unsigned u = __float_as_uint(x);
+  auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  u = __float_as_uint(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ unsigned uniform(unsigned x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// One work-group: one split of one sequence's tokens for one cache head and up
+// to 16 * kTiles of the query heads that share it.  Its wavefronts take steps of
+// 32 tokens in turn and join their sums through LDS at the end.
+//
+// kQ: the activations' type, kC: the cache's; kDim: head_dim rounded up to 64, 128
+// or 256.
+template <int kQ, int kC, int kDim, int kTiles>
+__global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendArgs a) {
+  constexpr bool kNarrow = kC == ROCSHMEM_AMD_E4M3;
+  // Scores multiply in the activations' type (e4m3 is exact in either), weights
+  // and values in the cache's, or in bf16 where the cache is e4m3: a value's scale
+  // is folded into its weight, which may then be as large or small as a scale.
+  constexpr int kP = kNarrow ? ROCSHMEM_AMD_BF16 : kC;
+  using QM = Mma<kQ>;
+  using PM = Mma<kP>;
+  constexpr int kBytes = kNarrow ? 1 : 2;
+  constexpr int kDots = kDim / 32;                // products along a row of keys
+  constexpr int kKeyLoads = kDim * kBytes / 64;   // 16-byte loads for a lane's share of a unit's keys
+  constexpr int kCols = kDim / 16;                // elements of a value row in a lane
+  constexpr int kWords = kCols * kBytes / 4;      // words they take
+  // Weights are kept 2^kLift above exp(s - maximum): the maximum is followed only
+  // once a score passes it by 2^kSlack, and fp16's smallest weights keep bits.
+  constexpr float kLift = kP == ROCSHMEM_AMD_HALF ? 7.f : 0.f, kSlack = 8.f;
+
+  __shared__ float sh_top[kAttendWaves][16 * kTiles], sh_sum[kAttendWaves][16 * kTiles];
+  __shared__ __attribute__((aligned(16))) float sh_out[kAttendWaves][16][kDim + 4];
+
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int column = lane & 15, quad = lane >> 4;
+  const int b = blockIdx.y, split = blockIdx.z;
+  const uint32_t head = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles;
+  const int head0 = head * a.group + tile * 16 * kTiles;
+  const int heads_here = a.group - static_cast<int>(tile) * 16 * kTiles < 16 * kTiles
+                             ? a.group - static_cast<int>(tile) * 16 * kTiles : 16 * kTiles;
+  const bool counts = blockIdx.x == 0 && wave == 0;
+
+  const Span span = span_of(a, b, counts && split == 0 && lane == 0);
+  const int first_unit = span.first_unit() + split * a.split_units;
+  const int end_unit = first_unit + a.split_units < span.end_unit() ? first_unit + a.split_units : span.end_unit();
+  if (first_unit >= end_unit && split > 0) return;
+  const bool whole = span.end_unit() - span.first_unit() <= a.split_units;  // no other split has any
+
+  // ---- the query, and where the lane's loads are from a unit's first row -----------
+  const uint32_t d = a.cache.head_dim, row_bytes = a.cache.row_bytes;
+  uint32_t key_at[kKeyLoads];
+#pragma unroll
+  for (int j = 0; j < kKeyLoads; ++j) {
+    const uint32_t at = j * 64 + quad * 16;  // beyond the row: its start again, against a zero of the query
+    key_at[j] = column * row_bytes + (at < row_bytes ? at : 0);
+  }
+  const uint32_t piece = column * kCols * kBytes;  // beyond the row: columns that nobody reads
+  const uint32_t value_at = 4 * quad * row_bytes + (piece < row_bytes ? piece : 0);
+  typename QM::V q[kTiles][kDots];
+#pragma unroll
+  for (int n = 0; n < kTiles; ++n) {
+    const int h = n * 16 + column;
+    const char *row = a.q + (b * a.q_row + static_cast<uint64_t>(head0 + (h < heads_here ? h : 0)) * d) * 2;
+#pragma unroll
+    for (int j = 0; j < kDots; ++j) {
+      const uint32_t e = kNarrow ? (j / 2) * 64 + quad * 16 + (j % 2) * 8 : j * 32 + quad * 8;
+      typename QM::V v{};
+      if (h < heads_here && e < d) v = load_loose<typename QM::V>(row + e * 2);
+      q[n][j] = v;
+    }
+  }
+
+  F4 acc[kTiles][kCols];
+  float top[kTiles], sum[kTiles];
+#pragma unroll
+  for (int n = 0; n < kTiles; ++n) {
+    top[n] = -INFINITY;
+    sum[n] = 0.f;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) acc[n][c] = F4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // ---- units of 16 tokens, 64 at a time, a lane for each ----------------------------
+  unsigned page_lo, page_hi, unit_row;
+  int unit_token, n_units;
+  const auto look_up = [&](int first) {
+    const int unit = first + lane;
+    bool there = unit < end_unit;
+    uint64_t page = 0;
+    uint32_t at = 0;
+    if (there) {
+      const uint32_t index = quotient(static_cast<uint32_t>(unit), a.cache.by_page_units);
+      at = static_cast<uint32_t>(unit) * 16 - index * a.cache.page_tokens;
+      const uint32_t number = static_cast<uint32_t>(a.page_table[b * a.table_row + index]);
+      if (number >= a.cache.n_pages) {
+        there = false;
+        if (counts && (at == 0 || unit == span.first_unit())) count_refused(a.refused);
+      } else {
+        const uint32_t pe = owner_of(a.cache, number);
+        there = !a.own_pages || static_cast<int>(pe) == a.my_pe;
+        page = reinterpret_cast<uint64_t>(detail::remote_addr(a.ctx, a.cache.pages, static_cast<int>(pe)) +
+                                          page_offset(a.cache, number, pe));
+      }
+    }
+    page_lo = static_cast<unsigned>(page);
+    page_hi = static_cast<unsigned>(page >> 32);
+    unit_row = head * a.cache.page_tokens + at;
+    unit_token = unit * 16;
+    // Close up over what takes no part: another PE's pages where only this one's
+    // count, page numbers out of range.
+    const uint64_t mask = __ballot(there);
+    n_units = __popcll(mask);
+    if (mask & (mask + 1)) {
+      const int before = __popcll(mask & ((uint64_t{1} << lane) - 1));
+      const int to = 4 * (there ? before : n_units + lane - before);
+      page_lo = __builtin_amdgcn_ds_permute(to, page_lo);
+      page_hi = __builtin_amdgcn_ds_permute(to, page_hi);
+      unit_row = __builtin_amdgcn_ds_permute(to, unit_row);
+      unit_token = __builtin_amdgcn_ds_permute(to, unit_token);
+    }
+  };
+
+  // ---- one step: two units ---------------------------------------------------------
+  U4 keys[2][kKeyLoads];
+  unsigned values[8][kWords], key_scales[2], value_scales[2];
+  const auto of_lane = [](unsigned x, int i) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(x, i)); };
+  // As global memory: an address put together from lanes would be read as flat
+  // memory, whose loads are waited for all at once.
+  const auto page_of = [&](int i) {
+    return (GlobalBytes)(of_lane(page_lo, i) | (static_cast<uint64_t>(of_lane(page_hi, i)) << 32));  // NOLINT
+  };
+  // An odd number of units: the last step's second one is the first again, left out by its weights.
+  const auto unit_of = [&](int step, int u) { return 2 * step + u < n_units ? 2 * step + u : 2 * step; };
+  const auto load_keys = [&](int step) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int i = unit_of(step, u);
+      const GlobalBytes page = page_of(i);
+      const uint32_t row = of_lane(unit_row, i);
+      const GlobalBytes from = page + static_cast<uint64_t>(row) * row_bytes;
+#pragma unroll
+      for (int j = 0; j < kKeyLoads; ++j) keys[u][j] = read_at<U4>(from, key_at[j]);
+      if constexpr (kNarrow) key_scales[u] = read_at<unsigned>(page + a.cache.key_scale_offset + row, 4 * quad);
+    }
+  };
+  const auto load_values = [&](int step) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int i = unit_of(step, u);
+      const GlobalBytes page = page_of(i);
+      const uint32_t row = of_lane(unit_row, i);
+      const GlobalBytes from = page + a.cache.value_offset + static_cast<uint64_t>(row) * row_bytes;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const uint32_t at = value_at + t * row_bytes;
+        if constexpr (kWords == 1) {
+          values[4 * u + t][0] = read_at<unsigned>(from, at);
+        } else if constexpr (kWords == 2) {
+          const U2 v = read_at<U2>(from, at);
+          values[4 * u + t][0] = v[0];
+          values[4 * u + t][1] = v[1];
+        } else {
+#pragma unroll
+          for (int w = 0; w < kWords; w += 4) {
+            const U4 v = read_at<U4>(from, at + 4 * w);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) values[4 * u + t][w + x] = v[x];
+          }
+        }
+      }
+      if constexpr (kNarrow) value_scales[u] = read_at<unsigned>(page + a.cache.value_scale_offset + row, 4 * quad);
+    }
+  };
+
+  typename PM::V weights[kTiles][2];  // rounded, and what the rounding left
+  const auto score = [&](F4 (&s)[kTiles][2]) {
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) s[n][u] = F4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int j = 0; j < kKeyLoads; ++j) {
+        if constexpr (kNarrow) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            U4 k;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              k[2 * w] = QM::template from_e4m3<false>(keys[u][j][2 * half + w]);
+              k[2 * w + 1] = QM::template from_e4m3<true>(keys[u][j][2 * half + w]);
+            }
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n)
+              s[n][u] = QM::mul(__builtin_bit_cast(typename QM::V, k), q[n][2 * j + half], s[n][u]);
+          }
+        } else {
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n)
+            s[n][u] = QM::mul(__builtin_bit_cast(typename QM::V, keys[u][j]), q[n][j], s[n][u]);
+        }
+      }
+  };
+  const auto weigh = [&](int step, F4 (&s)[kTiles][2], bool &cut, bool (&in)[2][4]) {
+    int token[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) token[u] = __builtin_amdgcn_readlane(unit_token, unit_of(step, u));
+    cut = 2 * step + 2 > n_units || token[0] < span.first || token[1] + 16 > span.end;
+    if (cut) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int t = token[u] + 4 * quad + r;
+          in[u][r] = t >= span.first && t < span.end && 2 * step + u < n_units;
+        }
+    }
+    float up[2][4];  // from a product to a score, base 2
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        up[u][r] = a.softcap > 0.f ? a.scale : a.scale * kLog2e;
+        if constexpr (kNarrow) up[u][r] *= two_to((key_scales[u] >> (8 * r)) & 0xff);
+      }
+    bool ahead = false;
+    float most[kTiles];
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[n][u][r] *= up[u][r];
+      if (a.softcap > 0.f) {
+        // cap tanh(x), x = s / cap:  tanh(x) = 1 - 2 / (e^2x + 1)
+        const float in_scale = 2.f * kLog2e / a.softcap;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float e = __builtin_amdgcn_exp2f(s[n][u][r] * in_scale);
+            s[n][u][r] = a.softcap * kLog2e * (1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f));
+          }
+      }
+      if (cut) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[n][u][r] = in[u][r] ? s[n][u][r] : -INFINITY;
+      }
+      most[n] = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) most[n] = fmaxf(most[n], s[n][u][r]);
+      ahead = ahead || most[n] > top[n] + kSlack;
+    }
+    if (__any(ahead)) {
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) {
+        const float next = fmaxf(top[n], max_of_column(most[n]));
+        const float keep = top[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top[n] - next);
+        sum[n] *= keep;
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) acc[n][c] *= keep;
+        top[n] = next;
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+      const float from = top[n] == -INFINITY ? 0.f : top[n] - kLift;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float p = __builtin_amdgcn_exp2f(s[n][u][r] - from);
+          sum[n] += p;
+          if constexpr (kNarrow) p *= two_to((value_scales[u] >> (8 * r)) & 0xff);
+          if (kNarrow && cut) p = in[u][r] ? p : 0.f;
+          const typename PM::E high = static_cast<typename PM::E>(p);
+          weights[n][0][4 * u + r] = high;
+          weights[n][1][4 * u + r] = static_cast<typename PM::E>(p - static_cast<float>(high));
+        }
+    }
+  };
+  const auto add_values = [&](bool cut, const bool (&in)[2][4]) {
+    if (cut) {  // what lies behind the last token may be anything
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int w = 0; w < kWords; ++w) values[4 * u + r][w] = in[u][r] ? values[4 * u + r][w] : 0u;
+    }
+#pragma unroll
+    for (int c = 0; c < kCols; c += 2) {
+      U4 even, odd;  // columns c and c + 1 of the lane's eight tokens
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        if constexpr (kNarrow) {
+          const unsigned both = __builtin_amdgcn_perm(values[2 * p + 1][c / 4], values[2 * p][c / 4],
+                                                      c % 4 ? 0x07030602u : 0x05010400u);
+          even[p] = PM::template from_e4m3<false>(both);
+          odd[p] = PM::template from_e4m3<true>(both);
+        } else {
+          even[p] = __builtin_amdgcn_perm(values[2 * p + 1][c / 2], values[2 * p][c / 2], 0x05040100u);
+          odd[p] = __builtin_amdgcn_perm(values[2 * p + 1][c / 2], values[2 * p][c / 2], 0x07060302u);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          acc[n][c] = PM::mul(__builtin_bit_cast(typename PM::V, even), weights[n][part], acc[n][c]);
+          acc[n][c + 1] = PM::mul(__builtin_bit_cast(typename PM::V, odd), weights[n][part], acc[n][c + 1]);
+        }
+    }
+  };
+
+  for (int first = first_unit; first < end_unit; first += 64) {
+    look_up(first);
+    const int steps = (n_units + 1) / 2;
+    int step = wave;
+    if (step >= steps) continue;
+    load_keys(step);
+    load_values(step);
+    F4 s[kTiles][2];
+    bool cut, in[2][4] = {};
+    // The next step's keys are asked for as soon as this one's are used up, its
+    // values likewise: one of the two is always on its way.  The last step stands
+    // by itself, so that no wait has to allow for loads that were not made.
+    for (; step + kAttendWaves < steps; step += kAttendWaves) {
+      score(s);
+      weigh(step, s, cut, in);
+      load_keys(step + kAttendWaves);
+      add_values(cut, in);
+      load_values(step + kAttendWaves);
+    }
+    score(s);
+    weigh(step, s, cut, in);
+    add_values(cut, in);
+  }
+
+  // ---- the wavefronts' sums joined -----------------------------------------------
+#pragma unroll
+  for (int n = 0; n < kTiles; ++n) {
+    sum[n] = sum_of_column(sum[n]);
+    if (quad == 0) {
+      sh_top[wave][n * 16 + column] = top[n] == -INFINITY ? -INFINITY : top[n] - kLift;
+      sh_sum[wave][n * 16 + column] = sum[n];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < kTiles; ++n) {
+    const int mine = n * 16 + column;
+    float most = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kAttendWaves; ++w) most = fmaxf(most, sh_top[w][mine]);
+    const float own_top = sh_top[wave][mine];
+    const float keep = own_top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(own_top - most);
+    if (n) __syncthreads();  // the tile before has been read
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int c = 0; c < kCols; c += 4)
+        *reinterpret_cast<F4 *>(&sh_out[wave][column][(4 * quad + r) * kCols + c]) =
+            F4{acc[n][c][r] * keep, acc[n][c + 1][r] * keep, acc[n][c + 2][r] * keep, acc[n][c + 3][r] * keep};
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * kDim / 8; i += 64 * kAttendWaves) {
+      const int h = i / (kDim / 8), e = i % (kDim / 8) * 8;
+      if (n * 16 + h >= heads_here || e >= static_cast<int>(d)) continue;
+      float from = -INFINITY, total = 0.f, x[8] = {};
+#pragma unroll
+      for (int w = 0; w < kAttendWaves; ++w) from = fmaxf(from, sh_top[w][n * 16 + h]);
+#pragma unroll
+      for (int w = 0; w < kAttendWaves; ++w) {
+        const float t = sh_top[w][n * 16 + h];
+        total += t == -INFINITY ? 0.f : sh_sum[w][n * 16 + h] * __builtin_amdgcn_exp2f(t - from);
+#pragma unroll
+        for (int y = 0; y < 8; ++y) x[y] += sh_out[w][h][e + y];
+      }
+      const uint64_t row = static_cast<uint64_t>(b) * a.q_heads + head0 + n * 16 + h;
+      if (whole) {
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+        for (int y = 0; y < 8; ++y) x[y] *= inv;
+        store_out(a, b, head0 + n * 16 + h, e, x);
+        if (e == 0 && a.lse) a.lse[row] = (from + __builtin_amdgcn_logf(total)) * kLn2;
+      } else {
+        const uint64_t at = row * a.splits + split;
+        Eight<ROCSHMEM_AMD_FLOAT>::store(reinterpret_cast<char *>(a.part + at * d + e),
+                                         Eight<ROCSHMEM_AMD_FLOAT>::round(x));
+        if (e == 0) a.part_stat[at] = F2{from, total};
+      }
+    }
+  }
+}
+
+}  // namespace kv
+}  // namespace rocshmem
+
+#endif  // ROCSHMEM_AMD_KV_ATTEND_HPP_
