@@ -6,14 +6,18 @@ namespace kv {
 
 // A call is cut so that there are about this many work-groups (six for each of
 // 256 CUs), each with at least one step for every wavefront.
-constexpr int64_t kWantedWorkGroups = 1536;
-constexpr int64_t kMaxSplits = 4096;
+constexpr int64_t kWantedWorkGroups = 1024;
+
+constexpr int kMostTokens = 1 << 27;  // 2^15 splits of the largest size
 
 // Joins a sequence's splits: out = sum_i 2^(t_i - t) o_i / sum_i 2^(t_i - t) l_i over the
 // splits that have tokens, t the largest t_i.  One work-group per sequence and
-// query head; 64 lanes along the row, the splits dealt out to the four wavefronts.
+// query head: kLanes lanes along the row, four elements each, and the splits dealt
+// out to the 256 / kLanes groups, four of a group's on their way at once.
+template <int kLanes>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
-  const int b = blockIdx.y, h = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int kGroups = 256 / kLanes, kAhead = 4;
+  const int b = blockIdx.y, h = blockIdx.x, lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   const Span span = span_of(a, b, false);
   const int units = span.end_unit() - span.first_unit();
   if (units <= a.split_units) return;  // its only split has written the result
@@ -21,35 +25,48 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
   const uint64_t row = static_cast<uint64_t>(b) * a.q_heads + h;
   const F2 *stat = a.part_stat + row * a.splits;
   const uint32_t d = a.cache.head_dim;
-  __shared__ float sh_top[4], sh_total[4];
-  __shared__ F4 sh_out[4][64];
+  const bool mine = lane * 4u < d;
+  const float *part = a.part + row * a.splits * d + (mine ? lane * 4 : 0);
+  __shared__ float sh_top[4], sh_total[kGroups];
+  __shared__ F4 sh_out[kGroups][kLanes];
   float top = -INFINITY;
   for (int i = threadIdx.x; i < n; i += 256) top = fmaxf(top, stat[i].x);
   for (int hop = 32; hop; hop /= 2) top = fmaxf(top, __shfl_xor(top, hop));
-  if (lane == 0) sh_top[wave] = top;
+  if (threadIdx.x % 64 == 0) sh_top[threadIdx.x / 64] = top;
   __syncthreads();
   top = fmaxf(fmaxf(sh_top[0], sh_top[1]), fmaxf(sh_top[2], sh_top[3]));
   const float from = top == -INFINITY ? 0.f : top;
   float total = 0.f;
   F4 x{0.f, 0.f, 0.f, 0.f};
-  for (int i = wave; i < n; i += 4) {
-    const F2 s = stat[i];
-    const float w = __builtin_amdgcn_exp2f(s.x - from);
-    total += w * s.y;
-    if (lane * 4u < d) x += w * *reinterpret_cast<const F4 *>(a.part + (row * a.splits + i) * d + lane * 4);
+  for (int i0 = group; i0 < n; i0 += kAhead * kGroups) {
+    F2 s[kAhead];
+    F4 o[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = i0 + k * kGroups, at = i < n ? i : i0;
+      s[k] = stat[at];
+      o[k] = *reinterpret_cast<const F4 *>(part + static_cast<uint64_t>(at) * d);
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const float w = i0 + k * kGroups < n ? __builtin_amdgcn_exp2f(s[k].x - from) : 0.f;
+      total += w * s[k].y;
+      x += w * o[k];
+    }
   }
-  sh_out[wave][lane] = x;
-  if (lane == 0) sh_total[wave] = total;
+  sh_out[group][lane] = x;
+  if (lane == 0) sh_total[group] = total;
   __syncthreads();
-  total = sh_total[0] + sh_total[1] + sh_total[2] + sh_total[3];
-  const float inv = total == 0.f ? 0.f : 1.f / total;
-  if (threadIdx.x * 8 < d) {
-    float y[8] = {};
-    for (int w = 0; w < 4; ++w)
-      for (int e = 0; e < 8; ++e) y[e] += sh_out[w][threadIdx.x * 2 + e / 4][e % 4];
-    for (int e = 0; e < 8; ++e) y[e] *= inv;
-    store_out(a, b, h, threadIdx.x * 8, y);
+  if (threadIdx.x * 8 >= d) return;
+  total = 0.f;
+  float y[8] = {};
+  for (int g = 0; g < kGroups; ++g) {
+    total += sh_total[g];
+    for (int e = 0; e < 8; ++e) y[e] += sh_out[g][threadIdx.x * 2 + e / 4][e % 4];
   }
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  for (int e = 0; e < 8; ++e) y[e] *= inv;
+  store_out(a, b, h, threadIdx.x * 8, y);
   if (a.lse && threadIdx.x == 0) a.lse[row] = (top + __builtin_amdgcn_logf(total)) * kLn2;
 }
 
@@ -63,9 +80,16 @@ static Cut cut_of(int64_t work_groups_per_split, int64_t max_tokens) {
   const int64_t wanted = (kWantedWorkGroups + work_groups_per_split - 1) / work_groups_per_split;
   int64_t each = (units + wanted - 1) / wanted;
   each = (each + 7) / 8 * 8;  // a step of every wavefront
-  if (each > 64) each = 64;
-  while ((units + each - 1) / each > kMaxSplits) each *= 2;
+  if (each > kMostUnits) each = kMostUnits;
   return Cut{static_cast<int>(each), static_cast<int>((units + each - 1) / each)};
+}
+// The most splits that a call of at most max_tokens can have, whatever its window.
+static int64_t most_splits(int64_t work_groups_per_split, int64_t max_tokens) {
+  const int64_t wanted = (kWantedWorkGroups + work_groups_per_split - 1) / work_groups_per_split;
+  const int64_t finest = ((max_tokens + 15) / 16 + 1 + 7) / 8;
+  const int64_t splits = cut_of(work_groups_per_split, max_tokens).splits;
+  const int64_t few = wanted < finest ? wanted : finest;
+  return splits > few ? splits : few;
 }
 static int columns_of(int group, int head_dim) {  // tiles of 16 query heads that one work-group takes
   const int tiles = (group + 15) / 16;
@@ -103,7 +127,13 @@ static void launch_attend(const AttendArgs &a, int n_seqs, hipStream_t s) {
     launch_columns<kQ, kC, 256>(a, columns, grid, s);
   DRV_CHECK_HIP(hipGetLastError());
   if (a.splits > 1) {
-    hipLaunchKernelGGL(attend_join_kernel, dim3(a.q_heads, n_seqs), dim3(256), 0, s, a);
+    const dim3 rows(a.q_heads, n_seqs);
+    if (a.cache.head_dim <= 64)
+      hipLaunchKernelGGL(attend_join_kernel<16>, rows, dim3(256), 0, s, a);
+    else if (a.cache.head_dim <= 128)
+      hipLaunchKernelGGL(attend_join_kernel<32>, rows, dim3(256), 0, s, a);
+    else
+      hipLaunchKernelGGL(attend_join_kernel<64>, rows, dim3(256), 0, s, a);
     DRV_CHECK_HIP(hipGetLastError());
   }
 }
@@ -119,11 +149,11 @@ extern "C" {
 size_t rocshmem_amd_kv_attend_bytes(const rocshmem_amd_kv_cache_t *cache, int n_seqs, int q_heads, int max_len) {
   Layout c;
   if (!cache || !fill_layout(cache->dtype, cache->page_tokens, cache->kv_heads, cache->head_dim, 1, 1, &c)) return 0;
-  if (n_seqs < 1 || n_seqs > 65535 || max_len < 1 || q_heads < 1 || q_heads > 65535 || q_heads % cache->kv_heads) return 0;
+  if (n_seqs < 1 || n_seqs > 65535 || max_len < 1 || max_len > kMostTokens || q_heads < 1 || q_heads > 65535 || q_heads % cache->kv_heads) return 0;
   const int group = q_heads / cache->kv_heads, columns = columns_of(group, cache->head_dim);
   const int64_t tiles = (group + 16 * columns - 1) / (16 * columns);
   return part_bytes(static_cast<size_t>(n_seqs) * q_heads,
-                    cut_of(n_seqs * tiles * cache->kv_heads, max_len).splits, c.head_dim);
+                    most_splits(n_seqs * tiles * cache->kv_heads, max_len), c.head_dim);
 }
 
 int rocshmem_amd_kv_attend(const rocshmem_amd_kv_cache_t *cache, int dtype, const void *q, size_t q_row,
@@ -138,7 +168,7 @@ int rocshmem_amd_kv_attend(const rocshmem_amd_kv_cache_t *cache, int dtype, cons
   if (cache->dtype != ROCSHMEM_AMD_E4M3 && cache->dtype != dtype) return -1;
   if (out_dtype != dtype && out_dtype != ROCSHMEM_AMD_FLOAT) return -1;
   if (pages_from != ROCSHMEM_AMD_KV_ALL_PAGES && pages_from != ROCSHMEM_AMD_KV_OWN_PAGES) return -1;
-  if (n_seqs < 0 || n_seqs > 65535 || max_len < 0 || window < 0) return -1;
+  if (n_seqs < 0 || n_seqs > 65535 || max_len < 0 || max_len > kMostTokens || window < 0) return -1;
   if (q_heads < 1 || q_heads % cache->kv_heads || q_heads > 65535) return -1;
   if (!__builtin_isfinite(scale) || !__builtin_isfinite(softcap) || softcap < 0.f) return -1;
   if (!n_seqs) return 0;
@@ -160,17 +190,13 @@ int rocshmem_amd_kv_attend(const rocshmem_amd_kv_cache_t *cache, int dtype, cons
   const int columns = columns_of(a.group, cache->head_dim);
   a.tiles = (a.group + 16 * columns - 1) / (16 * columns);
   const int64_t per_split = static_cast<int64_t>(n_seqs) * cache->kv_heads * a.tiles;
-  const size_t needed = part_bytes(rows, cut_of(per_split, max_len).splits, a.cache.head_dim);
+  const size_t needed = part_bytes(rows, most_splits(per_split, max_len), a.cache.head_dim);
   if (needed && (!workspace || !aligned_to(workspace, 16) || workspace_bytes < needed ||
                  !drv::local_ok(workspace, workspace_bytes)))
     return -1;
   const Cut cut = cut_of(per_split, window > 0 && window < max_len ? window : max_len);
   a.split_units = cut.units;
   a.splits = cut.splits;
-  while (part_bytes(rows, a.splits, a.cache.head_dim) > needed) {  // a window is cut no finer than the whole
-    a.split_units *= 2;
-    a.splits = (a.splits + 1) / 2;
-  }
   a.part = static_cast<float *>(workspace);
   a.part_stat = reinterpret_cast<F2 *>(a.part + rows * a.splits * a.cache.head_dim);
   a.out_dtype = out_dtype;

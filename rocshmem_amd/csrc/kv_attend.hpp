@@ -74,13 +74,28 @@ __device__ __forceinline__ void store_out(const AttendArgs &a, int b, int h, int
     Eight<ROCSHMEM_AMD_HALF>::store(a.out + at * 2, Eight<ROCSHMEM_AMD_HALF>::round(x));
 }
 
+// Global memory by its address space: an address put together from lanes would
+// otherwise be read as flat memory, whose loads are waited for all at once.
 typedef const __attribute__((address_space(1))) char *GlobalBytes;
+typedef __attribute__((address_space(3))) char *LdsBytes;
 template <typename V>
 __device__ __forceinline__ V read_at(GlobalBytes from, uint32_t offset) {
   return *(const __attribute__((address_space(1))) V *)(from + offset);  // NOLINT
 }
+// What is read once: not kept in the caches at the expense of the rest.
+template <typename V>
+__device__ __forceinline__ V stream_at(GlobalBytes from, uint32_t offset) {
+  return __builtin_nontemporal_load((const __attribute__((address_space(1))) V *)(from + offset));  // NOLINT
+}
+// 16 bytes a lane straight to LDS, lane l's at `to` + 16 l; counted like a load.
+__device__ __forceinline__ void stream_to_lds(GlobalBytes from, uint32_t offset, LdsBytes to) {
+  constexpr int kNonTemporal = 2;
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(from + offset),  // NOLINT
+                                   (__attribute__((address_space(3))) void *)to, 16, 0, kNonTemporal);
+}
 
 constexpr int kAttendWaves = 4;
+constexpr int kMostUnits = 64 * kAttendWaves;  // of a split: a lane for each of a wavefront's
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
@@ -129,14 +144,24 @@ __device__ __forceinline__ float sum_of_column(float x) {
 }
 __device__ __forceinline__ unsigned uniform(unsigned x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// Wavefronts a SIMD is to hold: as many as the registers allow without spilling.
+constexpr int waves_of(int cache, int dim, int tiles) {
+#ifdef KV_WAVES
+  return KV_WAVES;
+#else
+  if (dim == 128) return tiles == 1 ? 3 : tiles == 2 ? 2 : 1;
+  return dim == 256 && cache == ROCSHMEM_AMD_E4M3 && tiles == 1 ? 2 : 1;
+#endif
+}
+
 // One work-group: one split of one sequence's tokens for one cache head and up
-// to 16 * kTiles of the query heads that share it.  Its wavefronts take steps of
-// 32 tokens in turn and join their sums through LDS at the end.
+// to 16 * kTiles of the query heads that share it.  Its wavefronts share the
+// tokens out, take 32 at a step, and join their sums through LDS at the end.
 //
 // kQ: the activations' type, kC: the cache's; kDim: head_dim rounded up to 64, 128
 // or 256.
 template <int kQ, int kC, int kDim, int kTiles>
-__global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendArgs a) {
+__global__ __launch_bounds__(64 * kAttendWaves, waves_of(kC, kDim, kTiles)) void attend_kernel(AttendArgs a) {
   constexpr bool kNarrow = kC == ROCSHMEM_AMD_E4M3;
   // Scores multiply in the activations' type (e4m3 is exact in either), weights
   // and values in the cache's, or in bf16 where the cache is e4m3: a value's scale
@@ -153,8 +178,12 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendArgs a)
   // once a score passes it by 2^kSlack, and fp16's smallest weights keep bits.
   constexpr float kLift = kP == ROCSHMEM_AMD_HALF ? 7.f : 0.f, kSlack = 8.f;
 
+  constexpr int kUnitBytes = kKeyLoads * 1024;    // a unit's keys in LDS
   __shared__ float sh_top[kAttendWaves][16 * kTiles], sh_sum[kAttendWaves][16 * kTiles];
-  __shared__ __attribute__((aligned(16))) float sh_out[kAttendWaves][16][kDim + 4];
+  __shared__ union __attribute__((aligned(16))) {
+    char keys[kAttendWaves][2][kUnitBytes];       // each wavefront's next step
+    float out[kAttendWaves][16][kDim + 4];        // and at the end its sums
+  } sh;
 
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int column = lane & 15, quad = lane >> 4;
@@ -163,21 +192,80 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendArgs a)
   const int head0 = head * a.group + tile * 16 * kTiles;
   const int heads_here = a.group - static_cast<int>(tile) * 16 * kTiles < 16 * kTiles
                              ? a.group - static_cast<int>(tile) * 16 * kTiles : 16 * kTiles;
-  const bool counts = blockIdx.x == 0 && wave == 0;
 
-  const Span span = span_of(a, b, counts && split == 0 && lane == 0);
+  // ---- the tokens: this wavefront's units of 16, a lane for each -----------------------
+  // Without a window a unit's number does not depend on the sequence's length, and
+  // its entry of the page table is asked for before the length is known.
+  const int per_wave = a.split_units / kAttendWaves;  // even, at most 64
+  const int place = split * a.split_units + wave * per_wave + lane;
+  const auto entry_of = [&](int unit) {
+    const uint32_t index = quotient(static_cast<uint32_t>(unit), a.cache.by_page_units);
+    return index < a.table_row ? static_cast<uint32_t>(a.page_table[b * a.table_row + index]) : ~0u;
+  };
+  uint32_t number = a.window > 0 ? 0u : entry_of(place);
+  const Span span = span_of(a, b, blockIdx.x == 0 && split == 0 && threadIdx.x == 0);
   const int first_unit = span.first_unit() + split * a.split_units;
   const int end_unit = first_unit + a.split_units < span.end_unit() ? first_unit + a.split_units : span.end_unit();
   if (first_unit >= end_unit && split > 0) return;
   const bool whole = span.end_unit() - span.first_unit() <= a.split_units;  // no other split has any
 
+  unsigned page_lo, page_hi, unit_row;
+  int unit_token, n_units;
+  {
+    const int unit = span.first_unit() + place;
+    bool there = lane < per_wave && unit < end_unit;
+    if (a.window > 0 && there) number = entry_of(unit);
+    uint64_t page = 0;
+    uint32_t at = 0;
+    if (there) {
+      const uint32_t index = quotient(static_cast<uint32_t>(unit), a.cache.by_page_units);
+      at = static_cast<uint32_t>(unit) * 16 - index * a.cache.page_tokens;
+      if (number >= a.cache.n_pages) {
+        there = false;
+        if (blockIdx.x == 0 && (at == 0 || unit == span.first_unit())) count_refused(a.refused);
+      } else {
+        const uint32_t pe = owner_of(a.cache, number);
+        there = !a.own_pages || static_cast<int>(pe) == a.my_pe;
+        page = reinterpret_cast<uint64_t>(detail::remote_addr(a.ctx, a.cache.pages, static_cast<int>(pe)) +
+                                          page_offset(a.cache, number, pe));
+      }
+    }
+    page_lo = static_cast<unsigned>(page);
+    page_hi = static_cast<unsigned>(page >> 32);
+    unit_row = head * a.cache.page_tokens + at;
+    unit_token = unit * 16;
+    // Close up over what takes no part: another PE's pages where only this one's
+    // count, page numbers out of range.
+    const uint64_t mask = __ballot(there);
+    n_units = __popcll(mask);
+    if (mask & (mask + 1)) {
+      const int before = __popcll(mask & ((uint64_t{1} << lane) - 1));
+      const int to = 4 * (there ? before : n_units + lane - before);
+      page_lo = __builtin_amdgcn_ds_permute(to, page_lo);
+      page_hi = __builtin_amdgcn_ds_permute(to, page_hi);
+      unit_row = __builtin_amdgcn_ds_permute(to, unit_row);
+      unit_token = __builtin_amdgcn_ds_permute(to, unit_token);
+    }
+  }
+
   // ---- the query, and where the lane's loads are from a unit's first row -----------
-  const uint32_t d = a.cache.head_dim, row_bytes = a.cache.row_bytes;
-  uint32_t key_at[kKeyLoads];
+  // A unit's keys are one run of 16 rows.  They are fetched as they lie, 1 KiB at a
+  // time (fetched by the product's lanes, 64 bytes of 16 rows at a time, the same
+  // loop ran at 5.0 TB/s instead of 5.9), into LDS, where a lane finds its piece of
+  // one token's row.  Rows would start in the same banks there, so row r's 16-byte
+  // pieces lie turned by r: a piece's place comes from turning what is fetched.
+  const uint32_t d = a.cache.head_dim, row_bytes = a.cache.row_bytes, pieces = row_bytes / 16;
+  const auto turn = [&](uint32_t row) { return pieces < 16 ? row * pieces / 16 : row; };
+  uint32_t key_from[kKeyLoads], key_at[kKeyLoads];
 #pragma unroll
   for (int j = 0; j < kKeyLoads; ++j) {
-    const uint32_t at = j * 64 + quad * 16;  // beyond the row: its start again, against a zero of the query
-    key_at[j] = column * row_bytes + (at < row_bytes ? at : 0);
+    const uint32_t place = j * 64 + lane, row = place / pieces, p = place - row * pieces;
+    const uint32_t piece = p >= turn(row) ? p - turn(row) : p + pieces - turn(row);
+    key_from[j] = row < 16 ? row * row_bytes + piece * 16 : 0;  // beyond the unit: its start again
+    uint32_t want = 4 * j + quad;
+    if (want >= pieces) want = 0;  // beyond the row: its start again, against a zero of the query
+    want += turn(column);
+    key_at[j] = column * row_bytes + (want < pieces ? want : want - pieces) * 16;
   }
   const uint32_t piece = column * kCols * kBytes;  // beyond the row: columns that nobody reads
   const uint32_t value_at = 4 * quad * row_bytes + (piece < row_bytes ? piece : 0);
@@ -205,48 +293,7 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendArgs a)
     for (int c = 0; c < kCols; ++c) acc[n][c] = F4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // ---- units of 16 tokens, 64 at a time, a lane for each ----------------------------
-  unsigned page_lo, page_hi, unit_row;
-  int unit_token, n_units;
-  const auto look_up = [&](int first) {
-    const int unit = first + lane;
-    bool there = unit < end_unit;
-    uint64_t page = 0;
-    uint32_t at = 0;
-    if (there) {
-      const uint32_t index = quotient(static_cast<uint32_t>(unit), a.cache.by_page_units);
-      at = static_cast<uint32_t>(unit) * 16 - index * a.cache.page_tokens;
-      const uint32_t number = static_cast<uint32_t>(a.page_table[b * a.table_row + index]);
-      if (number >= a.cache.n_pages) {
-        there = false;
-        if (counts && (at == 0 || unit == span.first_unit())) count_refused(a.refused);
-      } else {
-        const uint32_t pe = owner_of(a.cache, number);
-        there = !a.own_pages || static_cast<int>(pe) == a.my_pe;
-        page = reinterpret_cast<uint64_t>(detail::remote_addr(a.ctx, a.cache.pages, static_cast<int>(pe)) +
-                                          page_offset(a.cache, number, pe));
-      }
-    }
-    page_lo = static_cast<unsigned>(page);
-    page_hi = static_cast<unsigned>(page >> 32);
-    unit_row = head * a.cache.page_tokens + at;
-    unit_token = unit * 16;
-    // Close up over what takes no part: another PE's pages where only this one's
-    // count, page numbers out of range.
-    const uint64_t mask = __ballot(there);
-    n_units = __popcll(mask);
-    if (mask & (mask + 1)) {
-      const int before = __popcll(mask & ((uint64_t{1} << lane) - 1));
-      const int to = 4 * (there ? before : n_units + lane - before);
-      page_lo = __builtin_amdgcn_ds_permute(to, page_lo);
-      page_hi = __builtin_amdgcn_ds_permute(to, page_hi);
-      unit_row = __builtin_amdgcn_ds_permute(to, unit_row);
-      unit_token = __builtin_amdgcn_ds_permute(to, unit_token);
-    }
-  };
-
   // ---- one step: two units ---------------------------------------------------------
-  U4 keys[2][kKeyLoads];
   unsigned values[8][kWords], key_scales[2], value_scales[2];
   const auto of_lane = [](unsigned x, int i) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(x, i)); };
   // As global memory: an address put together from lanes would be read as flat
@@ -256,6 +303,7 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendArgs a)
   };
   // An odd number of units: the last step's second one is the first again, left out by its weights.
   const auto unit_of = [&](int step, int u) { return 2 * step + u < n_units ? 2 * step + u : 2 * step; };
+  const auto my_keys = [&](int u) { return (LdsBytes)&sh.keys[wave][u][0]; };  // NOLINT
   const auto load_keys = [&](int step) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -264,7 +312,7 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendArgs a)
       const uint32_t row = of_lane(unit_row, i);
       const GlobalBytes from = page + static_cast<uint64_t>(row) * row_bytes;
 #pragma unroll
-      for (int j = 0; j < kKeyLoads; ++j) keys[u][j] = read_at<U4>(from, key_at[j]);
+      for (int j = 0; j < kKeyLoads; ++j) stream_to_lds(from, key_from[j], my_keys(u) + j * 1024);
       if constexpr (kNarrow) key_scales[u] = read_at<unsigned>(page + a.cache.key_scale_offset + row, 4 * quad);
     }
   };
@@ -279,15 +327,15 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendArgs a)
       for (int t = 0; t < 4; ++t) {
         const uint32_t at = value_at + t * row_bytes;
         if constexpr (kWords == 1) {
-          values[4 * u + t][0] = read_at<unsigned>(from, at);
+          values[4 * u + t][0] = stream_at<unsigned>(from, at);
         } else if constexpr (kWords == 2) {
-          const U2 v = read_at<U2>(from, at);
+          const U2 v = stream_at<U2>(from, at);
           values[4 * u + t][0] = v[0];
           values[4 * u + t][1] = v[1];
         } else {
 #pragma unroll
           for (int w = 0; w < kWords; w += 4) {
-            const U4 v = read_at<U4>(from, at + 4 * w);
+            const U4 v = stream_at<U4>(from, at + 4 * w);
 #pragma unroll
             for (int x = 0; x < 4; ++x) values[4 * u + t][w + x] = v[x];
           }
@@ -297,6 +345,7 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendArgs a)
     }
   };
 
+  constexpr int kOnlyLds = 0xc07f;     // s_waitcnt lgkmcnt(0), leaving loads on their way
   typename PM::V weights[kTiles][2];  // rounded, and what the rounding left
   const auto score = [&](F4 (&s)[kTiles][2]) {
 #pragma unroll
@@ -307,14 +356,15 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendArgs a)
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int j = 0; j < kKeyLoads; ++j) {
+        const U4 raw = *(const __attribute__((address_space(3))) U4 *)(my_keys(u) + key_at[j]);  // NOLINT
         if constexpr (kNarrow) {
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             U4 k;
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
-              k[2 * w] = QM::template from_e4m3<false>(keys[u][j][2 * half + w]);
-              k[2 * w + 1] = QM::template from_e4m3<true>(keys[u][j][2 * half + w]);
+              k[2 * w] = QM::template from_e4m3<false>(raw[2 * half + w]);
+              k[2 * w + 1] = QM::template from_e4m3<true>(raw[2 * half + w]);
             }
 #pragma unroll
             for (int n = 0; n < kTiles; ++n)
@@ -323,9 +373,23 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendArgs a)
         } else {
 #pragma unroll
           for (int n = 0; n < kTiles; ++n)
-            s[n][u] = QM::mul(__builtin_bit_cast(typename QM::V, keys[u][j]), q[n][j], s[n][u]);
+            s[n][u] = QM::mul(__builtin_bit_cast(typename QM::V, raw), q[n][j], s[n][u]);
         }
       }
+    const float by = a.softcap > 0.f ? a.scale : a.scale * kLog2e;  // to a score, base 2
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float up = by;
+        if constexpr (kNarrow) up *= two_to((key_scales[u] >> (8 * r)) & 0xff);
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) s[n][u][r] *= up;
+      }
+    // The keys in LDS have been read, and not only asked for, before the next ones
+    // may be fetched over them.
+    __builtin_amdgcn_s_waitcnt(kOnlyLds);
+    __builtin_amdgcn_sched_barrier(0);
   };
   const auto weigh = [&](int step, F4 (&s)[kTiles][2], bool &cut, bool (&in)[2][4]) {
     int token[2];
@@ -341,22 +405,10 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendArgs a)
           in[u][r] = t >= span.first && t < span.end && 2 * step + u < n_units;
         }
     }
-    float up[2][4];  // from a product to a score, base 2
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        up[u][r] = a.softcap > 0.f ? a.scale : a.scale * kLog2e;
-        if constexpr (kNarrow) up[u][r] *= two_to((key_scales[u] >> (8 * r)) & 0xff);
-      }
     bool ahead = false;
     float most[kTiles];
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[n][u][r] *= up[u][r];
       if (a.softcap > 0.f) {
         // cap tanh(x), x = s / cap:  tanh(x) = 1 - 2 / (e^2x + 1)
         const float in_scale = 2.f * kLog2e / a.softcap;
@@ -443,24 +495,22 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendArgs a)
     }
   };
 
-  for (int first = first_unit; first < end_unit; first += 64) {
-    look_up(first);
-    const int steps = (n_units + 1) / 2;
-    int step = wave;
-    if (step >= steps) continue;
-    load_keys(step);
-    load_values(step);
+  if (const int steps = (n_units + 1) / 2; steps > 0) {
     F4 s[kTiles][2];
     bool cut, in[2][4] = {};
-    // The next step's keys are asked for as soon as this one's are used up, its
-    // values likewise: one of the two is always on its way.  The last step stands
-    // by itself, so that no wait has to allow for loads that were not made.
-    for (; step + kAttendWaves < steps; step += kAttendWaves) {
+    load_keys(0);
+    load_values(0);
+    // The next step's keys are asked for as soon as this one's have been read, its
+    // values as soon as this one's are used up: one of the two is always on its
+    // way.  The last step stands by itself, so that no wait has to allow for loads
+    // that were not made.
+    int step = 0;
+    for (; step + 1 < steps; ++step) {
       score(s);
+      load_keys(step + 1);
       weigh(step, s, cut, in);
-      load_keys(step + kAttendWaves);
       add_values(cut, in);
-      load_values(step + kAttendWaves);
+      load_values(step + 1);
     }
     score(s);
     weigh(step, s, cut, in);
@@ -490,7 +540,7 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendArgs a)
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int c = 0; c < kCols; c += 4)
-        *reinterpret_cast<F4 *>(&sh_out[wave][column][(4 * quad + r) * kCols + c]) =
+        *reinterpret_cast<F4 *>(&sh.out[wave][column][(4 * quad + r) * kCols + c]) =
             F4{acc[n][c][r] * keep, acc[n][c + 1][r] * keep, acc[n][c + 2][r] * keep, acc[n][c + 3][r] * keep};
     __syncthreads();
     for (int i = threadIdx.x; i < 16 * kDim / 8; i += 64 * kAttendWaves) {
@@ -504,7 +554,7 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendArgs a)
         const float t = sh_top[w][n * 16 + h];
         total += t == -INFINITY ? 0.f : sh_sum[w][n * 16 + h] * __builtin_amdgcn_exp2f(t - from);
 #pragma unroll
-        for (int y = 0; y < 8; ++y) x[y] += sh_out[w][h][e + y];
+        for (int y = 0; y < 8; ++y) x[y] += sh.out[w][h][e + y];
       }
       const uint64_t row = static_cast<uint64_t>(b) * a.q_heads + head0 + n * 16 + h;
       if (whole) {
