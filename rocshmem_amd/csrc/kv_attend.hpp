@@ -146,12 +146,9 @@ __device__ __forceinline__ unsigned uniform(unsigned x) { return __builtin_amdgc
 
 // Wavefronts a SIMD is to hold: as many as the registers allow without spilling.
 constexpr int waves_of(int cache, int dim, int tiles) {
-#ifdef KV_WAVES
-  return KV_WAVES;
-#else
-  if (dim == 128) return tiles == 1 ? 3 : tiles == 2 ? 2 : 1;
-  return dim == 256 && cache == ROCSHMEM_AMD_E4M3 && tiles == 1 ? 2 : 1;
-#endif
+  if (dim == 64) return tiles == 1 ? 4 : tiles == 4 ? 2 : 3;
+  if (dim == 128) return tiles > 1 ? 2 : cache == ROCSHMEM_AMD_E4M3 ? 4 : 3;
+  return tiles > 1 ? 1 : 2;
 }
 
 // One work-group: one split of one sequence's tokens for one cache head and up
@@ -184,6 +181,10 @@ __global__ __launch_bounds__(64 * kAttendWaves, waves_of(kC, kDim, kTiles)) void
     char keys[kAttendWaves][2][kUnitBytes];       // each wavefront's next step
     float out[kAttendWaves][16][kDim + 4];        // and at the end its sums
   } sh;
+  // Several tiles' queries would take the registers of another wavefront: they lie
+  // in LDS, as the products' lanes hold them.
+  constexpr bool kQueryInLds = kTiles > 1;
+  __shared__ U4 sh_query[kQueryInLds ? kTiles : 1][kQueryInLds ? kDots : 1][64];
 
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int column = lane & 15, quad = lane >> 4;
@@ -269,9 +270,8 @@ __global__ __launch_bounds__(64 * kAttendWaves, waves_of(kC, kDim, kTiles)) void
   }
   const uint32_t piece = column * kCols * kBytes;  // beyond the row: columns that nobody reads
   const uint32_t value_at = 4 * quad * row_bytes + (piece < row_bytes ? piece : 0);
-  typename QM::V q[kTiles][kDots];
-#pragma unroll
-  for (int n = 0; n < kTiles; ++n) {
+  typename QM::V query[kDots];
+  for (int n = kQueryInLds ? wave : 0; n < kTiles; n += kAttendWaves) {
     const int h = n * 16 + column;
     const char *row = a.q + (b * a.q_row + static_cast<uint64_t>(head0 + (h < heads_here ? h : 0)) * d) * 2;
 #pragma unroll
@@ -279,7 +279,10 @@ __global__ __launch_bounds__(64 * kAttendWaves, waves_of(kC, kDim, kTiles)) void
       const uint32_t e = kNarrow ? (j / 2) * 64 + quad * 16 + (j % 2) * 8 : j * 32 + quad * 8;
       typename QM::V v{};
       if (h < heads_here && e < d) v = load_loose<typename QM::V>(row + e * 2);
-      q[n][j] = v;
+      if constexpr (kQueryInLds)
+        sh_query[n][j][lane] = __builtin_bit_cast(U4, v);
+      else
+        query[j] = v;
     }
   }
 
@@ -345,17 +348,40 @@ __global__ __launch_bounds__(64 * kAttendWaves, waves_of(kC, kDim, kTiles)) void
     }
   };
 
-  constexpr int kOnlyLds = 0xc07f;     // s_waitcnt lgkmcnt(0), leaving loads on their way
-  typename PM::V weights[kTiles][2];  // rounded, and what the rounding left
-  const auto score = [&](F4 (&s)[kTiles][2]) {
+  constexpr int kOnlyLds = 0xc07f;  // s_waitcnt lgkmcnt(0), leaving loads on their way
+  typedef typename PM::V Weights[2];  // rounded, and what the rounding left
+  struct Which {                      // of a step's tokens take part
+    bool cut, in[2][4];
+  };
+  const auto which_of = [&](int step) {
+    Which w{};
+    int token[2];
 #pragma unroll
-    for (int n = 0; n < kTiles; ++n)
+    for (int u = 0; u < 2; ++u) token[u] = __builtin_amdgcn_readlane(unit_token, unit_of(step, u));
+    w.cut = 2 * step + 2 > n_units || token[0] < span.first || token[1] + 16 > span.end;
+    if (w.cut) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) s[n][u] = F4{0.f, 0.f, 0.f, 0.f};
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+        for (int r = 0; r < 4; ++r) {
+          const int t = token[u] + 4 * quad + r;
+          w.in[u][r] = t >= span.first && t < span.end && 2 * step + u < n_units;
+        }
+    }
+    return w;
+  };
+  const auto score = [&](int n, F4 (&s)[2]) {
+    s[0] = s[1] = F4{0.f, 0.f, 0.f, 0.f};
+    const auto query_of = [&](int j) {
+      if constexpr (kQueryInLds)
+        return __builtin_bit_cast(typename QM::V, sh_query[n][j][lane]);
+      else
+        return query[j];
+    };
 #pragma unroll
-      for (int j = 0; j < kKeyLoads; ++j) {
+    for (int j = 0; j < kKeyLoads; ++j)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
         const U4 raw = *(const __attribute__((address_space(3))) U4 *)(my_keys(u) + key_at[j]);  // NOLINT
         if constexpr (kNarrow) {
 #pragma unroll
@@ -366,14 +392,10 @@ __global__ __launch_bounds__(64 * kAttendWaves, waves_of(kC, kDim, kTiles)) void
               k[2 * w] = QM::template from_e4m3<false>(raw[2 * half + w]);
               k[2 * w + 1] = QM::template from_e4m3<true>(raw[2 * half + w]);
             }
-#pragma unroll
-            for (int n = 0; n < kTiles; ++n)
-              s[n][u] = QM::mul(__builtin_bit_cast(typename QM::V, k), q[n][2 * j + half], s[n][u]);
+            s[u] = QM::mul(__builtin_bit_cast(typename QM::V, k), query_of(2 * j + half), s[u]);
           }
         } else {
-#pragma unroll
-          for (int n = 0; n < kTiles; ++n)
-            s[n][u] = QM::mul(__builtin_bit_cast(typename QM::V, raw), q[n][j], s[n][u]);
+          s[u] = QM::mul(__builtin_bit_cast(typename QM::V, raw), query_of(j), s[u]);
         }
       }
     const float by = a.softcap > 0.f ? a.scale : a.scale * kLog2e;  // to a score, base 2
@@ -383,138 +405,150 @@ __global__ __launch_bounds__(64 * kAttendWaves, waves_of(kC, kDim, kTiles)) void
       for (int r = 0; r < 4; ++r) {
         float up = by;
         if constexpr (kNarrow) up *= two_to((key_scales[u] >> (8 * r)) & 0xff);
-#pragma unroll
-        for (int n = 0; n < kTiles; ++n) s[n][u][r] *= up;
+        s[u][r] *= up;
       }
-    // The keys in LDS have been read, and not only asked for, before the next ones
-    // may be fetched over them.
+  };
+  // The keys in LDS have been read, and not only asked for, before the next ones
+  // may be fetched over them.
+  const auto keys_are_read = [&] {
     __builtin_amdgcn_s_waitcnt(kOnlyLds);
     __builtin_amdgcn_sched_barrier(0);
   };
-  const auto weigh = [&](int step, F4 (&s)[kTiles][2], bool &cut, bool (&in)[2][4]) {
-    int token[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) token[u] = __builtin_amdgcn_readlane(unit_token, unit_of(step, u));
-    cut = 2 * step + 2 > n_units || token[0] < span.first || token[1] + 16 > span.end;
-    if (cut) {
+  const auto weigh = [&](int n, const Which &which, F4 (&s)[2], Weights &weights) {
+    if (a.softcap > 0.f) {
+      // cap tanh(x), x = s / cap:  tanh(x) = 1 - 2 / (e^2x + 1)
+      const float in_scale = 2.f * kLog2e / a.softcap;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int t = token[u] + 4 * quad + r;
-          in[u][r] = t >= span.first && t < span.end && 2 * step + u < n_units;
+          const float e = __builtin_amdgcn_exp2f(s[u][r] * in_scale);
+          s[u][r] = a.softcap * kLog2e * (1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f));
         }
     }
-    bool ahead = false;
-    float most[kTiles];
-#pragma unroll
-    for (int n = 0; n < kTiles; ++n) {
-      if (a.softcap > 0.f) {
-        // cap tanh(x), x = s / cap:  tanh(x) = 1 - 2 / (e^2x + 1)
-        const float in_scale = 2.f * kLog2e / a.softcap;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float e = __builtin_amdgcn_exp2f(s[n][u][r] * in_scale);
-            s[n][u][r] = a.softcap * kLog2e * (1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f));
-          }
-      }
-      if (cut) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s[n][u][r] = in[u][r] ? s[n][u][r] : -INFINITY;
-      }
-      most[n] = -INFINITY;
+    if (which.cut) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) most[n] = fmaxf(most[n], s[n][u][r]);
-      ahead = ahead || most[n] > top[n] + kSlack;
+        for (int r = 0; r < 4; ++r) s[u][r] = which.in[u][r] ? s[u][r] : -INFINITY;
     }
-    if (__any(ahead)) {
+    float most = -INFINITY;
 #pragma unroll
-      for (int n = 0; n < kTiles; ++n) {
-        const float next = fmaxf(top[n], max_of_column(most[n]));
-        const float keep = top[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top[n] - next);
-        sum[n] *= keep;
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int c = 0; c < kCols; ++c) acc[n][c] *= keep;
-        top[n] = next;
-      }
+      for (int r = 0; r < 4; ++r) most = fmaxf(most, s[u][r]);
+    if (__any(most > top[n] + kSlack)) {
+      const float next = fmaxf(top[n], max_of_column(most));
+      const float keep = top[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top[n] - next);
+      sum[n] *= keep;
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) acc[n][c] *= keep;
+      top[n] = next;
     }
+    const float from = top[n] == -INFINITY ? 0.f : top[n] - kLift;
 #pragma unroll
-    for (int n = 0; n < kTiles; ++n) {
-      const float from = top[n] == -INFINITY ? 0.f : top[n] - kLift;
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float p = __builtin_amdgcn_exp2f(s[n][u][r] - from);
-          sum[n] += p;
-          if constexpr (kNarrow) p *= two_to((value_scales[u] >> (8 * r)) & 0xff);
-          if (kNarrow && cut) p = in[u][r] ? p : 0.f;
-          const typename PM::E high = static_cast<typename PM::E>(p);
-          weights[n][0][4 * u + r] = high;
-          weights[n][1][4 * u + r] = static_cast<typename PM::E>(p - static_cast<float>(high));
+      for (int r = 0; r < 4; ++r) {
+        float p = __builtin_amdgcn_exp2f(s[u][r] - from);
+        sum[n] += p;
+        if constexpr (kNarrow) {
+          p *= two_to((value_scales[u] >> (8 * r)) & 0xff);
+          if (which.cut) p = which.in[u][r] ? p : 0.f;
         }
-    }
+        const typename PM::E high = static_cast<typename PM::E>(p);
+        weights[0][4 * u + r] = high;
+        weights[1][4 * u + r] = static_cast<typename PM::E>(p - static_cast<float>(high));
+      }
   };
-  const auto add_values = [&](bool cut, const bool (&in)[2][4]) {
-    if (cut) {  // what lies behind the last token may be anything
+  const auto clear_values = [&](const Which &which) {  // what lies behind the last token may be anything
+    if (which.cut) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-          for (int w = 0; w < kWords; ++w) values[4 * u + r][w] = in[u][r] ? values[4 * u + r][w] : 0u;
-    }
-#pragma unroll
-    for (int c = 0; c < kCols; c += 2) {
-      U4 even, odd;  // columns c and c + 1 of the lane's eight tokens
-#pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        if constexpr (kNarrow) {
-          const unsigned both = __builtin_amdgcn_perm(values[2 * p + 1][c / 4], values[2 * p][c / 4],
-                                                      c % 4 ? 0x07030602u : 0x05010400u);
-          even[p] = PM::template from_e4m3<false>(both);
-          odd[p] = PM::template from_e4m3<true>(both);
-        } else {
-          even[p] = __builtin_amdgcn_perm(values[2 * p + 1][c / 2], values[2 * p][c / 2], 0x05040100u);
-          odd[p] = __builtin_amdgcn_perm(values[2 * p + 1][c / 2], values[2 * p][c / 2], 0x07060302u);
-        }
-      }
-#pragma unroll
-      for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-        for (int part = 0; part < 2; ++part) {
-          acc[n][c] = PM::mul(__builtin_bit_cast(typename PM::V, even), weights[n][part], acc[n][c]);
-          acc[n][c + 1] = PM::mul(__builtin_bit_cast(typename PM::V, odd), weights[n][part], acc[n][c + 1]);
-        }
+          for (int w = 0; w < kWords; ++w) values[4 * u + r][w] = which.in[u][r] ? values[4 * u + r][w] : 0u;
     }
   };
+  // Columns c and c + 1 of the lane's eight tokens, as the product takes them.
+  const auto pair_up = [&](int c, U4 &even, U4 &odd) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      if constexpr (kNarrow) {
+        const unsigned both = __builtin_amdgcn_perm(values[2 * p + 1][c / 4], values[2 * p][c / 4],
+                                                    c % 4 ? 0x07030602u : 0x05010400u);
+        even[p] = PM::template from_e4m3<false>(both);
+        odd[p] = PM::template from_e4m3<true>(both);
+      } else {
+        even[p] = __builtin_amdgcn_perm(values[2 * p + 1][c / 2], values[2 * p][c / 2], 0x05040100u);
+        odd[p] = __builtin_amdgcn_perm(values[2 * p + 1][c / 2], values[2 * p][c / 2], 0x07060302u);
+      }
+    }
+  };
+  const auto add_pair = [&](int n, int c, const U4 &even, const U4 &odd, const Weights &weights) {
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      acc[n][c] = PM::mul(__builtin_bit_cast(typename PM::V, even), weights[part], acc[n][c]);
+      acc[n][c + 1] = PM::mul(__builtin_bit_cast(typename PM::V, odd), weights[part], acc[n][c + 1]);
+    }
+  };
+  // One step, tile by tile.  The next step's keys are asked for as soon as this
+  // one's have been read, its values as soon as this one's are used up.
+  const auto take = [&](int step, bool more) __attribute__((always_inline)) {
+    const Which which = which_of(step);
+    F4 s[2];
+    Weights weights;
+    if constexpr (kTiles == 1) {
+      score(0, s);
+      if (more) {
+        keys_are_read();
+        load_keys(step + 1);
+      }
+      weigh(0, which, s, weights);
+      clear_values(which);
+#pragma unroll
+      for (int c = 0; c < kCols; c += 2) {
+        U4 even, odd;
+        pair_up(c, even, odd);
+        add_pair(0, c, even, odd, weights);
+      }
+    } else {
+      // Paired up once for all tiles, as far as the registers reach.
+      constexpr bool kOnce = kTiles < 4;
+      U4 columns[kOnce ? kCols : 2];
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) {
+        score(n, s);
+        if (n == kTiles - 1 && more) {
+          keys_are_read();
+          load_keys(step + 1);
+        }
+        weigh(n, which, s, weights);
+        if (n == 0) clear_values(which);
+#pragma unroll
+        for (int c = 0; c < kCols; c += 2) {
+          const int at = kOnce ? c : 0;
+          if (!kOnce || n == 0) pair_up(c, columns[at], columns[at + 1]);
+          add_pair(n, c, columns[at], columns[at + 1], weights);
+        }
+      }
+    }
+    if (more) load_values(step + 1);
+  };
 
-  if (const int steps = (n_units + 1) / 2; steps > 0) {
-    F4 s[kTiles][2];
-    bool cut, in[2][4] = {};
+  const int steps = (n_units + 1) / 2;
+  if (steps > 0) {
     load_keys(0);
     load_values(0);
-    // The next step's keys are asked for as soon as this one's have been read, its
-    // values as soon as this one's are used up: one of the two is always on its
-    // way.  The last step stands by itself, so that no wait has to allow for loads
-    // that were not made.
+  }
+  if constexpr (kQueryInLds) __syncthreads();
+  if (steps > 0) {
+    // The last step stands by itself, so that no wait has to allow for loads that
+    // were not made.
     int step = 0;
-    for (; step + 1 < steps; ++step) {
-      score(s);
-      load_keys(step + 1);
-      weigh(step, s, cut, in);
-      add_values(cut, in);
-      load_values(step + 1);
-    }
-    score(s);
-    weigh(step, s, cut, in);
-    add_values(cut, in);
+    for (; step + 1 < steps; ++step) take(step, true);
+    take(step, false);
   }
 
   // ---- the wavefronts' sums joined -----------------------------------------------
