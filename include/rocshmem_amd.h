@@ -747,7 +747,7 @@ int rocshmem_amd_kv_get(const rocshmem_amd_kv_cache_t *cache, int dtype, void *k
  * q: n_seqs x q_heads x head_dim of `dtype` (the cache's, or BF16 or HALF for an
  * E4M3 cache), sequence b's at q + b * q_row elements.  out: the same shape in
  * out_dtype (`dtype`, or FLOAT for partial results), rows out_row elements
- * apart (at least q_heads * head_dim).  lse: n_seqs x q_heads floats, or NULL.
+ * apart (at least q_heads * head_dim).  max_len: at most 2^25.  lse: n_seqs x q_heads floats, or NULL.
  * A length above max_len, or above what table_row pages hold, counts as that
  * (and is counted as refused); a negative one as 0 (the same).
  * workspace: device memory of at least rocshmem_amd_kv_attend_bytes bytes,

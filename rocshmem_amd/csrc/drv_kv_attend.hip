@@ -4,65 +4,80 @@
 namespace rocshmem {
 namespace kv {
 
-// A call is cut so that there are about this many work-groups (six for each of
-// 256 CUs), each with at least one step for every wavefront.
-constexpr int64_t kWantedWorkGroups = 1024;
-
-constexpr int kMostTokens = 1 << 27;  // 2^15 splits of the largest size
+// Splits are cut for about this many work-groups over all (two for each CU), each of
+// at least one step for every wavefront and at most so many bytes of the cache:
+// beyond that the last ones to end leave the GPU half empty.  Measured with 384 to
+// 3072 work-groups and 32 to 256 units: 2 sequences to 131072 tokens in e4m3 70 us
+// here, 77 with three times the splits (each costs its start and its end); 64
+// sequences to 4096 in bf16 95 us, 104 with splits of twice the bytes.
+constexpr int64_t kWantedWorkGroups = 512, kMostSplitBytes = 1 << 20;
+constexpr int kMostTokens = 1 << 25;  // of a sequence: 2^15 of the smallest splits that kMostSplitBytes gives
 
 // Joins a sequence's splits: out = sum_i 2^(t_i - t) o_i / sum_i 2^(t_i - t) l_i over the
 // splits that have tokens, t the largest t_i.  One work-group per sequence and
 // query head: kLanes lanes along the row, four elements each, and the splits dealt
-// out to the 256 / kLanes groups, four of a group's on their way at once.
+// out to the 256 / kLanes groups, four of a group's on their way at once.  Each
+// group keeps its own largest t_i as it goes, and the first four are asked for
+// before the length, which only says how many of them count.
 template <int kLanes>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
   constexpr int kGroups = 256 / kLanes, kAhead = 4;
   const int b = blockIdx.y, h = blockIdx.x, lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  const uint64_t row = static_cast<uint64_t>(b) * a.q_heads + h;
+  const F2 *stat = a.part_stat + row * a.splits;
+  const uint32_t d = a.cache.head_dim;
+  const float *part = a.part + row * a.splits * d + (lane * 4u < d ? lane * 4 : 0);
+  __shared__ F2 sh_stat[kGroups];
+  __shared__ F4 sh_out[kGroups][kLanes];
+  F2 s[kAhead];
+  F4 o[kAhead];
+  const auto load = [&](int i0) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = i0 + k * kGroups, at = i < a.splits ? i : 0;
+      s[k] = stat[at];
+      o[k] = *reinterpret_cast<const F4 *>(part + static_cast<uint64_t>(at) * d);
+    }
+  };
+  load(group);
   const Span span = span_of(a, b, false);
   const int units = span.end_unit() - span.first_unit();
   if (units <= a.split_units) return;  // its only split has written the result
   const int n = (units + a.split_units - 1) / a.split_units;
-  const uint64_t row = static_cast<uint64_t>(b) * a.q_heads + h;
-  const F2 *stat = a.part_stat + row * a.splits;
-  const uint32_t d = a.cache.head_dim;
-  const bool mine = lane * 4u < d;
-  const float *part = a.part + row * a.splits * d + (mine ? lane * 4 : 0);
-  __shared__ float sh_top[4], sh_total[kGroups];
-  __shared__ F4 sh_out[kGroups][kLanes];
-  float top = -INFINITY;
-  for (int i = threadIdx.x; i < n; i += 256) top = fmaxf(top, stat[i].x);
-  for (int hop = 32; hop; hop /= 2) top = fmaxf(top, __shfl_xor(top, hop));
-  if (threadIdx.x % 64 == 0) sh_top[threadIdx.x / 64] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(sh_top[0], sh_top[1]), fmaxf(sh_top[2], sh_top[3]));
-  const float from = top == -INFINITY ? 0.f : top;
-  float total = 0.f;
+  float top = -INFINITY, total = 0.f;
   F4 x{0.f, 0.f, 0.f, 0.f};
-  for (int i0 = group; i0 < n; i0 += kAhead * kGroups) {
-    F2 s[kAhead];
-    F4 o[kAhead];
+  for (int i0 = group; i0 < n;) {
+    float next = top;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (i0 + k * kGroups < n) next = fmaxf(next, s[k].x);
+    const float from = next == -INFINITY ? 0.f : next, keep = __builtin_amdgcn_exp2f(top - from);
+    total *= keep;
+    x *= keep;
+    top = next;
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      const int i = i0 + k * kGroups, at = i < n ? i : i0;
-      s[k] = stat[at];
-      o[k] = *reinterpret_cast<const F4 *>(part + static_cast<uint64_t>(at) * d);
-    }
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const float w = i0 + k * kGroups < n ? __builtin_amdgcn_exp2f(s[k].x - from) : 0.f;
+      if (i0 + k * kGroups >= n) continue;
+      const float w = __builtin_amdgcn_exp2f(s[k].x - from);
       total += w * s[k].y;
       x += w * o[k];
     }
+    i0 += kAhead * kGroups;
+    if (i0 < n) load(i0);
   }
   sh_out[group][lane] = x;
-  if (lane == 0) sh_total[group] = total;
+  if (lane == 0) sh_stat[group] = F2{top, total};
   __syncthreads();
   if (threadIdx.x * 8 >= d) return;
+  top = -INFINITY;
+  for (int g = 0; g < kGroups; ++g) top = fmaxf(top, sh_stat[g].x);
+  const float from = top == -INFINITY ? 0.f : top;
   total = 0.f;
   float y[8] = {};
   for (int g = 0; g < kGroups; ++g) {
-    total += sh_total[g];
-    for (int e = 0; e < 8; ++e) y[e] += sh_out[g][threadIdx.x * 2 + e / 4][e % 4];
+    const float w = __builtin_amdgcn_exp2f(sh_stat[g].x - from);
+    total += w * sh_stat[g].y;
+    for (int e = 0; e < 8; ++e) y[e] += w * sh_out[g][threadIdx.x * 2 + e / 4][e % 4];
   }
   const float inv = total == 0.f ? 0.f : 1.f / total;
   for (int e = 0; e < 8; ++e) y[e] *= inv;
@@ -75,56 +90,59 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
 struct Cut {
   int units, splits;
 };
-static Cut cut_of(int64_t work_groups_per_split, int64_t max_tokens) {
+static Cut cut_of(int64_t work_groups_per_split, int64_t max_tokens, int64_t token_bytes) {
   const int64_t units = (max_tokens + 15) / 16 + 1;  // a window may start inside a unit
+  if (units <= kWholeUnits) return Cut{static_cast<int>(units), 1};
   const int64_t wanted = (kWantedWorkGroups + work_groups_per_split - 1) / work_groups_per_split;
   int64_t each = (units + wanted - 1) / wanted;
-  each = (each + 7) / 8 * 8;  // a step of every wavefront
-  if (each > kMostUnits) each = kMostUnits;
+  const int64_t most = kMostSplitBytes / (16 * token_bytes) < kMostUnits ? kMostSplitBytes / (16 * token_bytes) : kMostUnits;
+  if (each > most) each = most;
+  if (each >= units) each = (units + 1) / 2;
+  each = (each + 7) / 8 * 8;
   return Cut{static_cast<int>(each), static_cast<int>((units + each - 1) / each)};
 }
 // The most splits that a call of at most max_tokens can have, whatever its window.
-static int64_t most_splits(int64_t work_groups_per_split, int64_t max_tokens) {
+static int64_t most_splits(int64_t work_groups_per_split, int64_t max_tokens, int64_t token_bytes) {
   const int64_t wanted = (kWantedWorkGroups + work_groups_per_split - 1) / work_groups_per_split;
   const int64_t finest = ((max_tokens + 15) / 16 + 1 + 7) / 8;
-  const int64_t splits = cut_of(work_groups_per_split, max_tokens).splits;
+  const int64_t splits = cut_of(work_groups_per_split, max_tokens, token_bytes).splits;
   const int64_t few = wanted < finest ? wanted : finest;
   return splits > few ? splits : few;
 }
 static int columns_of(int group, int head_dim) {  // tiles of 16 query heads that one work-group takes
-  const int tiles = (group + 15) / 16;
-  const int most = head_dim > 128 ? 2 : 4;
+  const int tiles = (group + 15) / 16, most = head_dim > 128 ? 1 : 4;
   return tiles < most ? tiles : most;
 }
 static size_t part_bytes(size_t rows, size_t splits, size_t head_dim) {
   return splits > 1 ? rows * splits * (head_dim + 2) * sizeof(float) : 0;
 }
 
+template <int kQ, int kC, int kDim, int kTiles>
+static void launch_one(const AttendArgs &a, int n_seqs, hipStream_t s) {
+  const dim3 grid(a.cache.kv_heads * a.tiles, n_seqs, a.splits);
+  if (a.splits == 1)
+    hipLaunchKernelGGL((attend_kernel<kQ, kC, kDim, kTiles, true>), grid, dim3(64 * kWholeWaves), 0, s, a);
+  else
+    hipLaunchKernelGGL((attend_kernel<kQ, kC, kDim, kTiles, false>), grid, dim3(64 * kSplitWaves), 0, s, a);
+}
 template <int kQ, int kC, int kDim>
-static void launch_columns(const AttendArgs &a, int columns, dim3 grid, hipStream_t s) {
-  const dim3 block(64 * kAttendWaves);
-  switch (columns) {
-    case 1: hipLaunchKernelGGL((attend_kernel<kQ, kC, kDim, 1>), grid, block, 0, s, a); return;
-    case 2: hipLaunchKernelGGL((attend_kernel<kQ, kC, kDim, 2>), grid, block, 0, s, a); return;
-    default: break;
-  }
+static void launch_columns(const AttendArgs &a, int n_seqs, int columns, hipStream_t s) {
   if constexpr (kDim <= 128) {
-    if (columns == 3)
-      hipLaunchKernelGGL((attend_kernel<kQ, kC, kDim, 3>), grid, block, 0, s, a);
-    else
-      hipLaunchKernelGGL((attend_kernel<kQ, kC, kDim, 4>), grid, block, 0, s, a);
+    if (columns == 2) return launch_one<kQ, kC, kDim, 2>(a, n_seqs, s);
+    if (columns == 3) return launch_one<kQ, kC, kDim, 3>(a, n_seqs, s);
+    if (columns == 4) return launch_one<kQ, kC, kDim, 4>(a, n_seqs, s);
   }
+  launch_one<kQ, kC, kDim, 1>(a, n_seqs, s);
 }
 template <int kQ, int kC>
 static void launch_attend(const AttendArgs &a, int n_seqs, hipStream_t s) {
   const int columns = columns_of(a.group, static_cast<int>(a.cache.head_dim));
-  const dim3 grid(a.cache.kv_heads * a.tiles, n_seqs, a.splits);
   if (a.cache.head_dim <= 64)
-    launch_columns<kQ, kC, 64>(a, columns, grid, s);
+    launch_columns<kQ, kC, 64>(a, n_seqs, columns, s);
   else if (a.cache.head_dim <= 128)
-    launch_columns<kQ, kC, 128>(a, columns, grid, s);
+    launch_columns<kQ, kC, 128>(a, n_seqs, columns, s);
   else
-    launch_columns<kQ, kC, 256>(a, columns, grid, s);
+    launch_columns<kQ, kC, 256>(a, n_seqs, columns, s);
   DRV_CHECK_HIP(hipGetLastError());
   if (a.splits > 1) {
     const dim3 rows(a.q_heads, n_seqs);
@@ -153,7 +171,7 @@ size_t rocshmem_amd_kv_attend_bytes(const rocshmem_amd_kv_cache_t *cache, int n_
   const int group = q_heads / cache->kv_heads, columns = columns_of(group, cache->head_dim);
   const int64_t tiles = (group + 16 * columns - 1) / (16 * columns);
   return part_bytes(static_cast<size_t>(n_seqs) * q_heads,
-                    most_splits(n_seqs * tiles * cache->kv_heads, max_len), c.head_dim);
+                    most_splits(n_seqs * tiles * cache->kv_heads, max_len, 2 * c.row_bytes), c.head_dim);
 }
 
 int rocshmem_amd_kv_attend(const rocshmem_amd_kv_cache_t *cache, int dtype, const void *q, size_t q_row,
@@ -190,11 +208,11 @@ int rocshmem_amd_kv_attend(const rocshmem_amd_kv_cache_t *cache, int dtype, cons
   const int columns = columns_of(a.group, cache->head_dim);
   a.tiles = (a.group + 16 * columns - 1) / (16 * columns);
   const int64_t per_split = static_cast<int64_t>(n_seqs) * cache->kv_heads * a.tiles;
-  const size_t needed = part_bytes(rows, most_splits(per_split, max_len), a.cache.head_dim);
+  const size_t needed = part_bytes(rows, most_splits(per_split, max_len, 2 * a.cache.row_bytes), a.cache.head_dim);
   if (needed && (!workspace || !aligned_to(workspace, 16) || workspace_bytes < needed ||
                  !drv::local_ok(workspace, workspace_bytes)))
     return -1;
-  const Cut cut = cut_of(per_split, window > 0 && window < max_len ? window : max_len);
+  const Cut cut = cut_of(per_split, window > 0 && window < max_len ? window : max_len, 2 * a.cache.row_bytes);
   a.split_units = cut.units;
   a.splits = cut.splits;
   a.part = static_cast<float *>(workspace);

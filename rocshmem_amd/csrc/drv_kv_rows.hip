@@ -6,6 +6,8 @@
 namespace rocshmem {
 namespace kv {
 
+constexpr uint64_t kManyRows = 1 << 15;
+
 struct RowsArgs {
   Layout cache;
   const detail::Context *ctx;
@@ -16,76 +18,134 @@ struct RowsArgs {
   uint64_t n_tokens;
 };
 
-// Where a token's row starts in its owner's slice, as this PE sees it; the page
-// start goes to `page_out`.  Null for a slot that is left out.
-__device__ __forceinline__ char *page_of_slot(const RowsArgs &a, int64_t slot, bool counts, Place *at) {
+// The page of a token's slot, as this PE sees it, and the token's place in it.
+// Null for a slot that is left out.
+__device__ __forceinline__ char *page_of_slot(const RowsArgs &a, int64_t slot, bool counts, uint32_t *at) {
   if (!slot_in_range(a.cache, slot)) {
     if (slot != -1 && counts) count_refused(a.refused);
     return nullptr;
   }
-  *at = place_of(a.cache, slot);
-  const uint32_t pe = owner_of(a.cache, at->page);
-  return detail::remote_addr(a.ctx, a.cache.pages, static_cast<int>(pe)) + page_offset(a.cache, at->page, pe);
+  const Place place = place_of(a.cache, slot);
+  const uint32_t pe = owner_of(a.cache, place.page);
+  *at = place.at;
+  return detail::remote_addr(a.ctx, a.cache.pages, static_cast<int>(pe)) + page_offset(a.cache, place.page, pe);
 }
 
-// A group of kLanes lanes moves one row of one token, eight elements a lane.
-// Work-group (x, y): row x of 2 * kv_heads (all keys, then all values), tokens
-// y * groups on.
-template <int kSide, int kCache, int kLanes, bool kPut>
+// A lane's share of a row: 16 bytes of the cache, eight elements of 16 bits or
+// sixteen of e4m3, as runs of eight.
+template <int kCache>
+constexpr int kRuns = kCache == ROCSHMEM_AMD_E4M3 ? 2 : 1;
+
+// A group of kLanes lanes moves one row of kAhead tokens, whose loads are all on
+// their way before the first is used.  Work-group (x, y): row x of 2 * kv_heads (all
+// keys, then all values) of the tokens from y * groups * kAhead on; the groups take
+// neighbouring tokens, so that the scale bytes of tokens in neighbouring slots
+// leave in one store.  Bound by the bytes moved: nothing but the row's largest
+// magnitude is computed, across its lanes.
+template <int kSide, int kCache, int kLanes, int kAhead, bool kPut>
 __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
-  constexpr int kGroups = 256 / kLanes;
+  constexpr int kGroups = 256 / kLanes, kEach = 8 * kRuns<kCache>;
+  constexpr bool kNarrow = kCache == ROCSHMEM_AMD_E4M3;
+  using Side = Eight<kSide>;
+  using Cached = Eight<kCache>;
   const bool value = blockIdx.x >= a.cache.kv_heads;
   const uint32_t head = value ? blockIdx.x - a.cache.kv_heads : blockIdx.x;
   const uint32_t lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
-  const bool mine = lane * 8 < a.cache.head_dim;
-  for (uint64_t t0 = static_cast<uint64_t>(blockIdx.y) * kGroups; t0 < a.n_tokens;
-       t0 += static_cast<uint64_t>(gridDim.y) * kGroups) {
-    const uint64_t t = t0 + group;
-    char *page = nullptr;
-    Place at{};
-    if (t < a.n_tokens) page = page_of_slot(a, a.slots[t], blockIdx.x == 0 && lane == 0, &at);
-    if (!page) continue;  // the whole group: its lanes agree
-    char *cached = page + row_offset(a.cache, head, at.at, value) + lane * 8 * Eight<kCache>::kBytes;
-    char *scale = page + scale_offset(a.cache, head, at.at, value);
-    char *side = a.side[value] + t * a.side_row[value] +
-                 (head * a.cache.head_dim + lane * 8) * Eight<kSide>::kBytes;
-    float x[8] = {};
-    if constexpr (kPut) {
-      typename Eight<kSide>::Raw raw{};
-      if (mine) raw = Eight<kSide>::load(side);
-      if constexpr (kSide == kCache) {
-        if (mine) Eight<kCache>::store(cached, raw);
-      } else {
-        Eight<kSide>::widen(raw, x);
-        if constexpr (kCache == ROCSHMEM_AMD_E4M3) {
-          unsigned top = 0;  // magnitudes of floats order like their bits
-          for (int i = 0; i < 8; ++i) {
-            const unsigned bits = __float_as_uint(x[i]) & 0x7fffffffu;
-            if (bits < 0x7f800000u && bits > top) top = bits;
-          }
-          for (int hop = kLanes / 2; hop; hop /= 2) {
-            const unsigned other = __shfl_xor(top, hop, kLanes);
-            top = other > top ? other : top;
-          }
-          const unsigned byte = scale_byte(top);
-          const float down = two_to(254 - byte);
-          for (int i = 0; i < 8; ++i)
-            x[i] = __builtin_isfinite(x[i]) ? x[i] * down : __builtin_nanf("");
-          if (lane == 0) *scale = static_cast<char>(byte);
-        }
-        if (mine) Eight<kCache>::store(cached, Eight<kCache>::round(x));
+  const bool mine = lane * kEach < a.cache.head_dim;
+  const uint32_t element = mine ? lane * kEach : 0;
+  char *const rows = a.side[value] + (head * a.cache.head_dim + element) * Side::kBytes;
+  for (uint64_t t0 = static_cast<uint64_t>(blockIdx.y) * kGroups * kAhead + group; t0 < a.n_tokens;
+       t0 += static_cast<uint64_t>(gridDim.y) * kGroups * kAhead) {
+    int64_t slot[kAhead];
+    typename Side::Raw side[kAhead][kRuns<kCache>];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const uint64_t t = t0 + k * kGroups;
+      slot[k] = t < a.n_tokens ? a.slots[t] : -1;
+      if constexpr (kPut) {  // a row is there whatever its slot
+        const char *from = rows + (t < a.n_tokens ? t : t0) * a.side_row[value];
+#pragma unroll
+        for (int r = 0; r < kRuns<kCache>; ++r) side[k][r] = Side::load(from + 8 * r * Side::kBytes);
       }
-    } else if (mine) {
-      const auto raw = Eight<kCache>::load(cached);
-      if constexpr (kSide == kCache) {
-        Eight<kSide>::store(side, raw);
-      } else {
-        Eight<kCache>::widen(raw, x);
-        if constexpr (kCache == ROCSHMEM_AMD_E4M3) {
-          const float up = two_to(static_cast<unsigned char>(*scale));
-          for (int i = 0; i < 8; ++i) x[i] *= up;
+    }
+    char *page[kAhead];
+    uint32_t at[kAhead] = {};
+    typename Cached::Raw cached[kAhead][kRuns<kCache>] = {};
+    unsigned byte[kAhead] = {};
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      page[k] = page_of_slot(a, slot[k], blockIdx.x == 0 && lane == 0, &at[k]);
+      if constexpr (!kPut) {
+        if (!page[k]) continue;
+        const char *from = page[k] + row_offset(a.cache, head, at[k], value) + element * Cached::kBytes;
+#pragma unroll
+        for (int r = 0; r < kRuns<kCache>; ++r) cached[k][r] = Cached::load(from + 8 * r * Cached::kBytes);
+        if constexpr (kNarrow)
+          byte[k] = static_cast<unsigned char>(page[k][scale_offset(a.cache, head, at[k], value)]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      float x[kRuns<kCache>][8];
+      if constexpr (kPut && kNarrow) {
+        unsigned top = 0;  // magnitudes of floats order like their bits
+#pragma unroll
+        for (int r = 0; r < kRuns<kCache>; ++r) {
+          Side::widen(side[k][r], x[r]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const unsigned bits = __float_as_uint(x[r][i]) & 0x7fffffffu;
+            top = bits < 0x7f800000u && bits > top ? bits : top;
+          }
         }
-        Eight<kSide>::store(side, Eight<kSide>::round(x));
+#pragma unroll
+        for (int hop = kLanes / 2; hop; hop /= 2) {
+          const unsigned other = __shfl_xor(top, hop, kLanes);
+          top = other > top ? other : top;
+        }
+        byte[k] = scale_byte(top);
+        const float down = two_to(254 - byte[k]);
+#pragma unroll
+        for (int r = 0; r < kRuns<kCache>; ++r)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            x[r][i] = __builtin_isfinite(x[r][i]) ? x[r][i] * down : __builtin_nanf("");
+      }
+      if (!page[k] || !mine) continue;
+      if constexpr (kPut) {
+        char *to = page[k] + row_offset(a.cache, head, at[k], value) + element * Cached::kBytes;
+        if constexpr (kSide == kCache) {
+          Cached::store(to, side[k][0]);
+        } else {
+          typename Cached::Raw raw[kRuns<kCache>];
+#pragma unroll
+          for (int r = 0; r < kRuns<kCache>; ++r) {
+            if constexpr (!kNarrow) Side::widen(side[k][r], x[r]);
+            raw[r] = Cached::round(x[r]);
+          }
+          if constexpr (kNarrow) {
+            store_loose(to, U4{raw[0][0], raw[0][1], raw[1][0], raw[1][1]});
+            if (lane == 0) page[k][scale_offset(a.cache, head, at[k], value)] = static_cast<char>(byte[k]);
+          } else {
+            Cached::store(to, raw[0]);
+          }
+        }
+      } else {
+        char *to = rows + (t0 + k * kGroups) * a.side_row[value];
+#pragma unroll
+        for (int r = 0; r < kRuns<kCache>; ++r) {
+          if constexpr (kSide == kCache) {
+            Side::store(to, cached[k][r]);
+          } else {
+            Cached::widen(cached[k][r], x[r]);
+            if constexpr (kNarrow) {
+              const float up = two_to(byte[k]);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) x[r][i] *= up;
+            }
+            Side::store(to + 8 * r * Side::kBytes, Side::round(x[r]));
+          }
+        }
       }
     }
   }
@@ -93,19 +153,27 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
 
 template <int kSide, int kCache, bool kPut>
 static void launch_rows(const RowsArgs &a, hipStream_t s) {
-  const auto go = [&](auto lanes) {
-    constexpr int kLanes = decltype(lanes)::value;
-    const uint64_t chunks = (a.n_tokens + 256 / kLanes - 1) / (256 / kLanes);
+  const auto go = [&](auto lanes, auto ahead) {
+    constexpr int kLanes = decltype(lanes)::value, kAhead = decltype(ahead)::value;
+    constexpr uint64_t kTokens = 256 / kLanes * kAhead;
+    const uint64_t chunks = (a.n_tokens + kTokens - 1) / kTokens;
     const dim3 grid(2 * a.cache.kv_heads, static_cast<unsigned>(chunks < 65535 ? chunks : 65535));
-    hipLaunchKernelGGL((rows_kernel<kSide, kCache, kLanes, kPut>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((rows_kernel<kSide, kCache, kLanes, kAhead, kPut>), grid, dim3(256), 0, s, a);
   };
-  const uint32_t d = a.cache.head_dim;
-  if (d <= 64)
-    go(std::integral_constant<int, 8>{});
-  else if (d <= 128)
-    go(std::integral_constant<int, 16>{});
+  constexpr int kMost = kMaxHeadDim / (8 * kRuns<kCache>);
+  // Several tokens a group once there are enough of them to fill the GPU that way.
+  const auto lanes = [&](auto ahead) {
+    if (a.cache.head_dim <= 64)
+      go(std::integral_constant<int, kMost / 4>{}, ahead);
+    else if (a.cache.head_dim <= 128)
+      go(std::integral_constant<int, kMost / 2>{}, ahead);
+    else
+      go(std::integral_constant<int, kMost>{}, ahead);
+  };
+  if (a.n_tokens * a.cache.kv_heads >= kManyRows)
+    lanes(std::integral_constant<int, 4>{});
   else
-    go(std::integral_constant<int, 32>{});
+    lanes(std::integral_constant<int, 1>{});
   DRV_CHECK_HIP(hipGetLastError());
 }
 

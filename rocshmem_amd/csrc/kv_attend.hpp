@@ -94,8 +94,11 @@ __device__ __forceinline__ void stream_to_lds(GlobalBytes from, uint32_t offset,
                                    (__attribute__((address_space(3))) void *)to, 16, 0, kNonTemporal);
 }
 
-constexpr int kAttendWaves = 4;
-constexpr int kMostUnits = 64 * kAttendWaves;  // of a split: a lane for each of a wavefront's
+// Short sequences take a work-group of eight wavefronts each and no second kernel;
+// longer ones are split over work-groups of four.
+constexpr int kSplitWaves = 4, kWholeWaves = 8;
+constexpr int kMostUnits = 64 * kSplitWaves;  // of a split: a lane for each of a wavefront's
+constexpr int kWholeUnits = 32;               // of the longest sequence that is not split: two steps a wavefront
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
@@ -148,7 +151,7 @@ __device__ __forceinline__ unsigned uniform(unsigned x) { return __builtin_amdgc
 constexpr int waves_of(int cache, int dim, int tiles) {
   if (dim == 64) return tiles == 1 ? 4 : tiles == 4 ? 2 : 3;
   if (dim == 128) return tiles > 1 ? 2 : cache == ROCSHMEM_AMD_E4M3 ? 4 : 3;
-  return tiles > 1 ? 1 : 2;
+  return 2;
 }
 
 // One work-group: one split of one sequence's tokens for one cache head and up
@@ -156,9 +159,11 @@ constexpr int waves_of(int cache, int dim, int tiles) {
 // tokens out, take 32 at a step, and join their sums through LDS at the end.
 //
 // kQ: the activations' type, kC: the cache's; kDim: head_dim rounded up to 64, 128
-// or 256.
-template <int kQ, int kC, int kDim, int kTiles>
-__global__ __launch_bounds__(64 * kAttendWaves, waves_of(kC, kDim, kTiles)) void attend_kernel(AttendArgs a) {
+// or 256; kWhole: one split.
+template <int kQ, int kC, int kDim, int kTiles, bool kWhole>
+__global__ __launch_bounds__(64 * (kWhole ? kWholeWaves : kSplitWaves), kWhole ? 2 : waves_of(kC, kDim, kTiles))
+void attend_kernel(AttendArgs a) {
+  constexpr int kAttendWaves = kWhole ? kWholeWaves : kSplitWaves;
   constexpr bool kNarrow = kC == ROCSHMEM_AMD_E4M3;
   // Scores multiply in the activations' type (e4m3 is exact in either), weights
   // and values in the cache's, or in bf16 where the cache is e4m3: a value's scale
@@ -197,7 +202,7 @@ __global__ __launch_bounds__(64 * kAttendWaves, waves_of(kC, kDim, kTiles)) void
   // ---- the tokens: this wavefront's units of 16, a lane for each -----------------------
   // Without a window a unit's number does not depend on the sequence's length, and
   // its entry of the page table is asked for before the length is known.
-  const int per_wave = a.split_units / kAttendWaves;  // even, at most 64
+  const int per_wave = (a.split_units + 2 * kAttendWaves - 1) / (2 * kAttendWaves) * 2;  // at most 64
   const int place = split * a.split_units + wave * per_wave + lane;
   const auto entry_of = [&](int unit) {
     const uint32_t index = quotient(static_cast<uint32_t>(unit), a.cache.by_page_units);
@@ -515,7 +520,7 @@ __global__ __launch_bounds__(64 * kAttendWaves, waves_of(kC, kDim, kTiles)) void
       }
     } else {
       // Paired up once for all tiles, as far as the registers reach.
-      constexpr bool kOnce = kTiles < 4;
+      constexpr bool kOnce = kTiles < 3;
       U4 columns[kOnce ? kCols : 2];
 #pragma unroll
       for (int n = 0; n < kTiles; ++n) {
