@@ -6,8 +6,6 @@
 namespace rocshmem {
 namespace kv {
 
-constexpr uint64_t kManyRows = 1 << 15;
-
 struct RowsArgs {
   Layout cache;
   const detail::Context *ctx;
@@ -36,13 +34,15 @@ __device__ __forceinline__ char *page_of_slot(const RowsArgs &a, int64_t slot, b
 template <int kCache>
 constexpr int kRuns = kCache == ROCSHMEM_AMD_E4M3 ? 2 : 1;
 
-// A group of kLanes lanes moves one row of kAhead tokens, whose loads are all on
-// their way before the first is used.  Work-group (x, y): row x of 2 * kv_heads (all
-// keys, then all values) of the tokens from y * groups * kAhead on; the groups take
-// neighbouring tokens, so that the scale bytes of tokens in neighbouring slots
-// leave in one store.  Bound by the bytes moved: nothing but the row's largest
-// magnitude is computed, across its lanes.
-template <int kSide, int kCache, int kLanes, int kAhead, bool kPut>
+// A group of kLanes lanes moves one row of one token.  Work-group (x, y): row x of
+// 2 * kv_heads (all keys, then all values) of 256 / kLanes neighbouring tokens, so that
+// the scale bytes of tokens in neighbouring slots leave in one store.  Bound by the
+// bytes moved: nothing but the row's largest magnitude is computed, across its
+// lanes.  65536 tokens of 8 heads x 128, 16-bit rows 12 KiB apart to and from e4m3:
+// put 94 us, get 73 us into and out of consecutive slots (4.3 and 5.5 TB/s), 99 and
+// 86 us scattered; two, four or eight tokens a group, all loads ahead, took 3 to 12 %
+// longer, and whole tokens a work-group instead of one head the same time.
+template <int kSide, int kCache, int kLanes, bool kPut>
 __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
   constexpr int kGroups = 256 / kLanes, kEach = 8 * kRuns<kCache>;
   constexpr bool kNarrow = kCache == ROCSHMEM_AMD_E4M3;
@@ -54,97 +54,72 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
   const bool mine = lane * kEach < a.cache.head_dim;
   const uint32_t element = mine ? lane * kEach : 0;
   char *const rows = a.side[value] + (head * a.cache.head_dim + element) * Side::kBytes;
-  for (uint64_t t0 = static_cast<uint64_t>(blockIdx.y) * kGroups * kAhead + group; t0 < a.n_tokens;
-       t0 += static_cast<uint64_t>(gridDim.y) * kGroups * kAhead) {
-    int64_t slot[kAhead];
-    typename Side::Raw side[kAhead][kRuns<kCache>];
+  for (uint64_t t = static_cast<uint64_t>(blockIdx.y) * kGroups + group; t < a.n_tokens;
+       t += static_cast<uint64_t>(gridDim.y) * kGroups) {
+    const int64_t slot = a.slots[t];
+    char *const row = rows + t * a.side_row[value];
+    typename Side::Raw side[kRuns<kCache>];
+    if constexpr (kPut) {  // the row is there whatever its slot
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const uint64_t t = t0 + k * kGroups;
-      slot[k] = t < a.n_tokens ? a.slots[t] : -1;
-      if constexpr (kPut) {  // a row is there whatever its slot
-        const char *from = rows + (t < a.n_tokens ? t : t0) * a.side_row[value];
-#pragma unroll
-        for (int r = 0; r < kRuns<kCache>; ++r) side[k][r] = Side::load(from + 8 * r * Side::kBytes);
-      }
+      for (int r = 0; r < kRuns<kCache>; ++r) side[r] = Side::load(row + 8 * r * Side::kBytes);
     }
-    char *page[kAhead];
-    uint32_t at[kAhead] = {};
-    typename Cached::Raw cached[kAhead][kRuns<kCache>] = {};
-    unsigned byte[kAhead] = {};
+    uint32_t at = 0;
+    char *const page = page_of_slot(a, slot, blockIdx.x == 0 && lane == 0, &at);
+    if (!page) continue;  // the whole group: its lanes agree
+    char *const cached = page + row_offset(a.cache, head, at, value) + element * Cached::kBytes;
+    char *const scale = page + scale_offset(a.cache, head, at, value);
+    float x[kRuns<kCache>][8];
+    if constexpr (kPut && kSide == kCache) {
+      if (mine) Cached::store(cached, side[0]);
+    } else if constexpr (kPut && !kNarrow) {
+      Side::widen(side[0], x[0]);
+      if (mine) Cached::store(cached, Cached::round(x[0]));
+    } else if constexpr (kPut) {
+      unsigned top = 0;  // magnitudes of floats order like their bits
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      page[k] = page_of_slot(a, slot[k], blockIdx.x == 0 && lane == 0, &at[k]);
-      if constexpr (!kPut) {
-        if (!page[k]) continue;
-        const char *from = page[k] + row_offset(a.cache, head, at[k], value) + element * Cached::kBytes;
+      for (int r = 0; r < kRuns<kCache>; ++r) {
+        Side::widen(side[r], x[r]);
 #pragma unroll
-        for (int r = 0; r < kRuns<kCache>; ++r) cached[k][r] = Cached::load(from + 8 * r * Cached::kBytes);
-        if constexpr (kNarrow)
-          byte[k] = static_cast<unsigned char>(page[k][scale_offset(a.cache, head, at[k], value)]);
+        for (int i = 0; i < 8; ++i) {
+          const unsigned bits = __float_as_uint(x[r][i]) & 0x7fffffffu;
+          top = bits < 0x7f800000u && bits > top ? bits : top;
+        }
       }
-    }
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      float x[kRuns<kCache>][8];
-      if constexpr (kPut && kNarrow) {
-        unsigned top = 0;  // magnitudes of floats order like their bits
-#pragma unroll
-        for (int r = 0; r < kRuns<kCache>; ++r) {
-          Side::widen(side[k][r], x[r]);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const unsigned bits = __float_as_uint(x[r][i]) & 0x7fffffffu;
-            top = bits < 0x7f800000u && bits > top ? bits : top;
-          }
-        }
-#pragma unroll
-        for (int hop = kLanes / 2; hop; hop /= 2) {
-          const unsigned other = __shfl_xor(top, hop, kLanes);
-          top = other > top ? other : top;
-        }
-        byte[k] = scale_byte(top);
-        const float down = two_to(254 - byte[k]);
-#pragma unroll
-        for (int r = 0; r < kRuns<kCache>; ++r)
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            x[r][i] = __builtin_isfinite(x[r][i]) ? x[r][i] * down : __builtin_nanf("");
+      for (int hop = kLanes / 2; hop; hop /= 2) {
+        const unsigned other = __shfl_xor(top, hop, kLanes);
+        top = other > top ? other : top;
       }
-      if (!page[k] || !mine) continue;
-      if constexpr (kPut) {
-        char *to = page[k] + row_offset(a.cache, head, at[k], value) + element * Cached::kBytes;
-        if constexpr (kSide == kCache) {
-          Cached::store(to, side[k][0]);
-        } else {
-          typename Cached::Raw raw[kRuns<kCache>];
+      const unsigned byte = scale_byte(top);
+      const float down = two_to(254 - byte);
+      U4 codes;
 #pragma unroll
-          for (int r = 0; r < kRuns<kCache>; ++r) {
-            if constexpr (!kNarrow) Side::widen(side[k][r], x[r]);
-            raw[r] = Cached::round(x[r]);
-          }
-          if constexpr (kNarrow) {
-            store_loose(to, U4{raw[0][0], raw[0][1], raw[1][0], raw[1][1]});
-            if (lane == 0) page[k][scale_offset(a.cache, head, at[k], value)] = static_cast<char>(byte[k]);
-          } else {
-            Cached::store(to, raw[0]);
-          }
-        }
+      for (int r = 0; r < kRuns<kCache>; ++r) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          x[r][i] = __builtin_isfinite(x[r][i]) ? x[r][i] * down : __builtin_nanf("");
+        const U2 raw = Cached::round(x[r]);
+        codes[2 * r] = raw[0];
+        codes[2 * r + 1] = raw[1];
+      }
+      if (mine) store_loose(cached, codes);
+      if (lane == 0) *scale = static_cast<char>(byte);
+    } else if (mine) {
+      typename Cached::Raw raw[kRuns<kCache>];
+#pragma unroll
+      for (int r = 0; r < kRuns<kCache>; ++r) raw[r] = Cached::load(cached + 8 * r * Cached::kBytes);
+      if constexpr (kSide == kCache) {
+        Side::store(row, raw[0]);
       } else {
-        char *to = rows + (t0 + k * kGroups) * a.side_row[value];
+        const float up = kNarrow ? two_to(static_cast<unsigned char>(*scale)) : 1.f;
 #pragma unroll
         for (int r = 0; r < kRuns<kCache>; ++r) {
-          if constexpr (kSide == kCache) {
-            Side::store(to, cached[k][r]);
-          } else {
-            Cached::widen(cached[k][r], x[r]);
-            if constexpr (kNarrow) {
-              const float up = two_to(byte[k]);
+          Cached::widen(raw[r], x[r]);
+          if constexpr (kNarrow) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i) x[r][i] *= up;
-            }
-            Side::store(to + 8 * r * Side::kBytes, Side::round(x[r]));
+            for (int i = 0; i < 8; ++i) x[r][i] *= up;
           }
+          Side::store(row + 8 * r * Side::kBytes, Side::round(x[r]));
         }
       }
     }
@@ -153,27 +128,19 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
 
 template <int kSide, int kCache, bool kPut>
 static void launch_rows(const RowsArgs &a, hipStream_t s) {
-  const auto go = [&](auto lanes, auto ahead) {
-    constexpr int kLanes = decltype(lanes)::value, kAhead = decltype(ahead)::value;
-    constexpr uint64_t kTokens = 256 / kLanes * kAhead;
-    const uint64_t chunks = (a.n_tokens + kTokens - 1) / kTokens;
+  const auto go = [&](auto lanes) {
+    constexpr int kLanes = decltype(lanes)::value;
+    const uint64_t chunks = (a.n_tokens + 256 / kLanes - 1) / (256 / kLanes);
     const dim3 grid(2 * a.cache.kv_heads, static_cast<unsigned>(chunks < 65535 ? chunks : 65535));
-    hipLaunchKernelGGL((rows_kernel<kSide, kCache, kLanes, kAhead, kPut>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((rows_kernel<kSide, kCache, kLanes, kPut>), grid, dim3(256), 0, s, a);
   };
   constexpr int kMost = kMaxHeadDim / (8 * kRuns<kCache>);
-  // Several tokens a group once there are enough of them to fill the GPU that way.
-  const auto lanes = [&](auto ahead) {
-    if (a.cache.head_dim <= 64)
-      go(std::integral_constant<int, kMost / 4>{}, ahead);
-    else if (a.cache.head_dim <= 128)
-      go(std::integral_constant<int, kMost / 2>{}, ahead);
-    else
-      go(std::integral_constant<int, kMost>{}, ahead);
-  };
-  if (a.n_tokens * a.cache.kv_heads >= kManyRows)
-    lanes(std::integral_constant<int, 4>{});
+  if (a.cache.head_dim <= 64)
+    go(std::integral_constant<int, kMost / 4>{});
+  else if (a.cache.head_dim <= 128)
+    go(std::integral_constant<int, kMost / 2>{});
   else
-    lanes(std::integral_constant<int, 1>{});
+    go(std::integral_constant<int, kMost>{});
   DRV_CHECK_HIP(hipGetLastError());
 }
 
@@ -224,37 +191,93 @@ struct JoinArgs {
   const float *partial_lse;
   char *out;
   float *lse;
-  uint64_t n_pieces;  // rows * pieces per row
-  uint32_t pieces;    // of eight elements, per row
+  uint64_t n_pieces;  // 16 bytes of the partial results each
+  uint32_t pieces;    // per row
+  Divisor by_pieces;
   int first, stride, members;
 };
 
-// A lane joins eight elements of a row: two walks over the members, for the
-// largest lse and for the sums.
-template <int kIn, int kOut>
+// 16 bytes of a type as 32-bit values, and as many values of another type stored.
+template <int kType>
+struct Piece {
+  static constexpr int kEach = 8;
+  __device__ __forceinline__ static void load(const char *p, float (&x)[8]) {
+    Eight<kType>::widen(__builtin_nontemporal_load(reinterpret_cast<const typename Eight<kType>::Raw *>(p)), x);
+  }
+};
+template <>
+struct Piece<ROCSHMEM_AMD_FLOAT> {
+  static constexpr int kEach = 4;
+  __device__ __forceinline__ static void load(const char *p, float (&x)[4]) {
+    const F4 v = __builtin_nontemporal_load(reinterpret_cast<const F4 *>(p));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = v[i];
+  }
+};
+template <int kType>
+__device__ __forceinline__ void store_values(char *p, const float (&x)[8]) {
+  Eight<kType>::store(p, Eight<kType>::round(x));
+}
+template <int kType>
+__device__ __forceinline__ void store_values(char *p, const float (&x)[4]) {
+  typedef __bf16 B4 __attribute__((ext_vector_type(4)));
+  typedef _Float16 H4 __attribute__((ext_vector_type(4)));
+  if constexpr (kType == ROCSHMEM_AMD_FLOAT)
+    store_loose(p, F4{x[0], x[1], x[2], x[3]});
+  else if constexpr (kType == ROCSHMEM_AMD_BF16)
+    store_loose(p, B4{static_cast<__bf16>(x[0]), static_cast<__bf16>(x[1]), static_cast<__bf16>(x[2]),
+                      static_cast<__bf16>(x[3])});
+  else
+    store_loose(p, H4{static_cast<_Float16>(x[0]), static_cast<_Float16>(x[1]), static_cast<_Float16>(x[2]),
+                      static_cast<_Float16>(x[3])});
+}
+
+// A lane joins 16 bytes of a row.  kAtOnce members' pieces and lse's are on their
+// way together; with more members the largest lse is followed from one such batch
+// to the next.
+template <int kIn, int kOut, int kAtOnce>
 __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
+  constexpr int kEach = Piece<kIn>::kEach;
   const uint64_t step = static_cast<uint64_t>(gridDim.x) * 256;
   for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x; i < a.n_pieces; i += step) {
-    const uint64_t row = i / a.pieces;
-    float top = -INFINITY;
-    for (int m = 0; m < a.members; ++m)
-      top = fmaxf(top, detail::remote_addr(a.ctx, a.partial_lse, a.first + m * a.stride)[row]);
-    const float from = top == -INFINITY ? 0.f : top;
-    float total = 0.f, sum[8] = {};
-    for (int m = 0; m < a.members; ++m) {
-      const int pe = a.first + m * a.stride;
-      const float lse = detail::remote_addr(a.ctx, a.partial_lse, pe)[row];
-      if (lse == -INFINITY) continue;
-      const float w = expf(lse - from);
-      float x[8];
-      Eight<kIn>::widen(Eight<kIn>::load(detail::remote_addr(a.ctx, a.partial, pe) + i * 8 * Eight<kIn>::kBytes), x);
-      total += w;
-      for (int e = 0; e < 8; ++e) sum[e] += w * x[e];
+    const uint64_t row = i >> 31 ? i / a.pieces : quotient(static_cast<uint32_t>(i), a.by_pieces);
+    float top = -INFINITY, total = 0.f, sum[kEach] = {};
+    for (int m0 = 0; m0 < a.members; m0 += kAtOnce) {
+      float lse[kAtOnce], x[kAtOnce][kEach];
+#pragma unroll
+      for (int m = 0; m < kAtOnce; ++m) {
+        const int pe = a.first + (m0 + m < a.members ? m0 + m : 0) * a.stride;
+        lse[m] = detail::remote_addr(a.ctx, a.partial_lse, pe)[row];
+        Piece<kIn>::load(detail::remote_addr(a.ctx, a.partial, pe) + i * 16, x[m]);
+      }
+      float next = top;
+#pragma unroll
+      for (int m = 0; m < kAtOnce; ++m) {
+        if (m0 + m >= a.members) lse[m] = -INFINITY;
+        next = fmaxf(next, lse[m]);
+      }
+      const float from = next == -INFINITY ? 0.f : next;
+      if (m0) {
+        const float keep = __builtin_amdgcn_exp2f((top - from) * kLog2e);
+        total *= keep;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) sum[e] *= keep;
+      }
+      top = next;
+#pragma unroll
+      for (int m = 0; m < kAtOnce; ++m) {
+        // exactly 0 without tokens, whatever the member's row holds then
+        const float w = __builtin_amdgcn_exp2f((lse[m] - from) * kLog2e);
+        total += w;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) sum[e] += lse[m] == -INFINITY ? 0.f : w * x[m][e];
+      }
     }
     const float inv = total == 0.f ? 0.f : 1.f / total;
-    for (int e = 0; e < 8; ++e) sum[e] *= inv;
-    Eight<kOut>::store(a.out + i * 8 * Eight<kOut>::kBytes, Eight<kOut>::round(sum));
-    if (a.lse && i == row * a.pieces) a.lse[row] = top + logf(total);
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) sum[e] *= inv;
+    store_values<kOut>(a.out + i * kEach * Eight<kOut>::kBytes, sum);
+    if (a.lse && i == row * a.pieces) a.lse[row] = top + __builtin_amdgcn_logf(total) * kLn2;
   }
 }
 
@@ -330,7 +353,8 @@ int rocshmem_amd_kv_join(int dtype, const void *partial, const float *partial_ls
   a.partial_lse = partial_lse;
   a.out = static_cast<char *>(out);
   a.lse = lse;
-  a.pieces = static_cast<uint32_t>(head_dim / 8);
+  a.pieces = static_cast<uint32_t>(d * es / 16);
+  a.by_pieces = make_divisor(a.pieces);
   a.n_pieces = n_rows * a.pieces;
   a.first = PE_start;
   a.stride = 1 << logPE_stride;
@@ -338,18 +362,20 @@ int rocshmem_amd_kv_join(int dtype, const void *partial, const float *partial_ls
   const uint64_t wgs = (a.n_pieces + 255) / 256;
   const dim3 grid(static_cast<unsigned>(wgs < (1u << 20) ? wgs : (1u << 20)));
   hipStream_t s = drv::as_stream(stream);
+  const auto go = [&](auto in, auto to) {
+    constexpr int kIn = decltype(in)::value, kOut = decltype(to)::value;
+    if (PE_size <= 2)
+      hipLaunchKernelGGL((join_kernel<kIn, kOut, 2>), grid, dim3(256), 0, s, a);
+    else if (PE_size <= 4)
+      hipLaunchKernelGGL((join_kernel<kIn, kOut, 4>), grid, dim3(256), 0, s, a);
+    else
+      hipLaunchKernelGGL((join_kernel<kIn, kOut, 8>), grid, dim3(256), 0, s, a);
+  };
   const auto to = [&](auto in) {
-    constexpr int kIn = decltype(in)::value;
     switch (out_dtype) {
-      case ROCSHMEM_AMD_BF16:
-        hipLaunchKernelGGL((join_kernel<kIn, ROCSHMEM_AMD_BF16>), grid, dim3(256), 0, s, a);
-        break;
-      case ROCSHMEM_AMD_HALF:
-        hipLaunchKernelGGL((join_kernel<kIn, ROCSHMEM_AMD_HALF>), grid, dim3(256), 0, s, a);
-        break;
-      default:
-        hipLaunchKernelGGL((join_kernel<kIn, ROCSHMEM_AMD_FLOAT>), grid, dim3(256), 0, s, a);
-        break;
+      case ROCSHMEM_AMD_BF16: go(in, std::integral_constant<int, ROCSHMEM_AMD_BF16>{}); break;
+      case ROCSHMEM_AMD_HALF: go(in, std::integral_constant<int, ROCSHMEM_AMD_HALF>{}); break;
+      default: go(in, std::integral_constant<int, ROCSHMEM_AMD_FLOAT>{}); break;
     }
   };
   switch (dtype) {

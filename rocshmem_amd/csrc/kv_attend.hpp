@@ -99,9 +99,6 @@ __device__ __forceinline__ void stream_to_lds(GlobalBytes from, uint32_t offset,
 constexpr int kSplitWaves = 4, kWholeWaves = 8;
 constexpr int kMostUnits = 64 * kSplitWaves;  // of a split: a lane for each of a wavefront's
 constexpr int kWholeUnits = 32;               // of the longest sequence that is not split: two steps a wavefront
-constexpr float kLog2e = 1.44269504088896340736f;
-constexpr float kLn2 = 0.69314718055994530942f;
-
 // The matrix product of a type, and pairs of values rounded to it.
 template <int kType>
 struct Mma;

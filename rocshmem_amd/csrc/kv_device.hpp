@@ -16,6 +16,9 @@ typedef float F4 __attribute__((ext_vector_type(4)));
 typedef __bf16 B8 __attribute__((ext_vector_type(8)));
 typedef _Float16 H8 __attribute__((ext_vector_type(8)));
 
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
 // A vector at any address its elements allow: gfx950's global loads and stores
 // need no more, and the compiler must not assume more.
 template <typename V>
