@@ -4,13 +4,17 @@
 namespace rocshmem {
 namespace kv {
 
-// Splits are cut for about this many work-groups over all (two for each CU), each of
-// at least one step for every wavefront and at most so many bytes of the cache:
-// beyond that the last ones to end leave the GPU half empty.  Measured with 384 to
-// 3072 work-groups and 32 to 256 units: 2 sequences to 131072 tokens in e4m3 70 us
-// here, 77 with three times the splits (each costs its start and its end); 64
-// sequences to 4096 in bf16 95 us, 104 with splits of twice the bytes.
+// Splits are cut for about this many work-groups over all (two for each CU), and of at
+// most so many bytes of the cache; the second half of the longest sequence into
+// splits a third as long.  Work-groups start in the order of their numbers, so the
+// short ones fill the gaps at the end, where a CU with one long split more than the
+// others would be waited for (a CU takes little more than its share of the memory's
+// rate, so a split too many on it is not made up for).  Measured, us, with equal
+// splits / with a half in thirds: 64 sequences to 4096 bf16 93.9 / 90.0, 48 heads on one
+// 52.4 / 45.3, 16 sequences with own heads 27.3 / 25.8, 2 to 131072 e4m3 69.2 / 68.8;
+// 1024 work-groups instead of 512: 90, 58, 26, 73; splits of 2 MiB: 105 for the first.
 constexpr int64_t kWantedWorkGroups = 512, kMostSplitBytes = 1 << 20;
+constexpr int64_t kLeastUnits = 16;  // of a short split: two steps of its wavefronts
 constexpr int kMostTokens = 1 << 25;  // of a sequence: 2^15 of the smallest splits that kMostSplitBytes gives
 
 // Joins a sequence's splits: out = sum_i 2^(t_i - t) o_i / sum_i 2^(t_i - t) l_i over the
@@ -24,9 +28,9 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
   constexpr int kGroups = 256 / kLanes, kAhead = 4;
   const int b = blockIdx.y, h = blockIdx.x, lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   const uint64_t row = static_cast<uint64_t>(b) * a.q_heads + h;
-  const F2 *stat = a.part_stat + row * a.splits;
+  const F2 *stat = a.part_stat + row * a.splits.most;
   const uint32_t d = a.cache.head_dim;
-  const float *part = a.part + row * a.splits * d + (lane * 4u < d ? lane * 4 : 0);
+  const float *part = a.part + row * a.splits.most * d + (lane * 4u < d ? lane * 4 : 0);
   __shared__ F2 sh_stat[kGroups];
   __shared__ F4 sh_out[kGroups][kLanes];
   F2 s[kAhead];
@@ -34,7 +38,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
   const auto load = [&](int i0) {
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      const int i = i0 + k * kGroups, at = i < a.splits ? i : 0;
+      const int i = i0 + k * kGroups, at = i < a.splits.most ? i : 0;
       s[k] = stat[at];
       o[k] = *reinterpret_cast<const F4 *>(part + static_cast<uint64_t>(at) * d);
     }
@@ -42,8 +46,8 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
   load(group);
   const Span span = span_of(a, b, false);
   const int units = span.end_unit() - span.first_unit();
-  if (units <= a.split_units) return;  // its only split has written the result
-  const int n = (units + a.split_units - 1) / a.split_units;
+  const int n = a.splits.count(units);
+  if (n <= 1) return;  // its only split has written the result
   float top = -INFINITY, total = 0.f;
   F4 x{0.f, 0.f, 0.f, 0.f};
   for (int i0 = group; i0 < n;) {
@@ -85,29 +89,26 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
   if (a.lse && threadIdx.x == 0) a.lse[row] = (top + __builtin_amdgcn_logf(total)) * kLn2;
 }
 
-// How a call is cut: tokens of a split (in units of 16) and how many splits the
-// longest sequence can have.
-struct Cut {
-  int units, splits;
-};
-static Cut cut_of(int64_t work_groups_per_split, int64_t max_tokens, int64_t token_bytes) {
+// How a call is cut: at most `limit` splits for the longest sequence.
+static Splits cut_of(int64_t work_groups_per_split, int64_t max_tokens, int64_t token_bytes, int limit) {
   const int64_t units = (max_tokens + 15) / 16 + 1;  // a window may start inside a unit
-  if (units <= kWholeUnits) return Cut{static_cast<int>(units), 1};
+  if (units <= kWholeUnits) return Splits{static_cast<int>(units), 1, 1, 1};
+  const auto whole_steps = [](int64_t n) { return (n + 2 * kSplitWaves - 1) / (2 * kSplitWaves) * (2 * kSplitWaves); };
   const int64_t wanted = (kWantedWorkGroups + work_groups_per_split - 1) / work_groups_per_split;
-  int64_t each = (units + wanted - 1) / wanted;
   const int64_t most = kMostSplitBytes / (16 * token_bytes) < kMostUnits ? kMostSplitBytes / (16 * token_bytes) : kMostUnits;
-  if (each > most) each = most;
-  if (each >= units) each = (units + 1) / 2;
-  each = (each + 7) / 8 * 8;
-  return Cut{static_cast<int>(each), static_cast<int>((units + each - 1) / each)};
-}
-// The most splits that a call of at most max_tokens can have, whatever its window.
-static int64_t most_splits(int64_t work_groups_per_split, int64_t max_tokens, int64_t token_bytes) {
-  const int64_t wanted = (kWantedWorkGroups + work_groups_per_split - 1) / work_groups_per_split;
-  const int64_t finest = ((max_tokens + 15) / 16 + 1 + 7) / 8;
-  const int64_t splits = cut_of(work_groups_per_split, max_tokens, token_bytes).splits;
-  const int64_t few = wanted < finest ? wanted : finest;
-  return splits > few ? splits : few;
+  int64_t big = (units + wanted - 1) / wanted;
+  if (big > most) big = most;
+  if (big >= units) big = (units + 1) / 2;
+  big = whole_steps(big);
+  int64_t small = whole_steps(big / 3 > kLeastUnits ? big / 3 : kLeastUnits);
+  for (;;) {
+    const int64_t n_big = units / 2 / big > 1 ? units / 2 / big : 1;
+    Splits s{static_cast<int>(big), static_cast<int>(n_big), static_cast<int>(small), 0};
+    s.most = s.count(static_cast<int>(units));
+    if (s.most <= limit || small >= kMostUnits) return s;
+    big = 2 * big < kMostUnits ? 2 * big : kMostUnits;
+    small = 2 * small < kMostUnits ? 2 * small : kMostUnits;
+  }
 }
 static int columns_of(int group, int head_dim) {  // tiles of 16 query heads that one work-group takes
   const int tiles = (group + 15) / 16, most = head_dim > 128 ? 1 : 4;
@@ -119,8 +120,8 @@ static size_t part_bytes(size_t rows, size_t splits, size_t head_dim) {
 
 template <int kQ, int kC, int kDim, int kTiles>
 static void launch_one(const AttendArgs &a, int n_seqs, hipStream_t s) {
-  const dim3 grid(a.cache.kv_heads * a.tiles, n_seqs, a.splits);
-  if (a.splits == 1)
+  const dim3 grid(a.cache.kv_heads * a.tiles, n_seqs, a.splits.most);
+  if (a.splits.most == 1)
     hipLaunchKernelGGL((attend_kernel<kQ, kC, kDim, kTiles, true>), grid, dim3(64 * kWholeWaves), 0, s, a);
   else
     hipLaunchKernelGGL((attend_kernel<kQ, kC, kDim, kTiles, false>), grid, dim3(64 * kSplitWaves), 0, s, a);
@@ -144,7 +145,7 @@ static void launch_attend(const AttendArgs &a, int n_seqs, hipStream_t s) {
   else
     launch_columns<kQ, kC, 256>(a, n_seqs, columns, s);
   DRV_CHECK_HIP(hipGetLastError());
-  if (a.splits > 1) {
+  if (a.splits.most > 1) {
     const dim3 rows(a.q_heads, n_seqs);
     if (a.cache.head_dim <= 64)
       hipLaunchKernelGGL(attend_join_kernel<16>, rows, dim3(256), 0, s, a);
@@ -171,7 +172,7 @@ size_t rocshmem_amd_kv_attend_bytes(const rocshmem_amd_kv_cache_t *cache, int n_
   const int group = q_heads / cache->kv_heads, columns = columns_of(group, cache->head_dim);
   const int64_t tiles = (group + 16 * columns - 1) / (16 * columns);
   return part_bytes(static_cast<size_t>(n_seqs) * q_heads,
-                    most_splits(n_seqs * tiles * cache->kv_heads, max_len, 2 * c.row_bytes), c.head_dim);
+                    cut_of(n_seqs * tiles * cache->kv_heads, max_len, 2 * c.row_bytes, INT32_MAX).most, c.head_dim);
 }
 
 int rocshmem_amd_kv_attend(const rocshmem_amd_kv_cache_t *cache, int dtype, const void *q, size_t q_row,
@@ -208,15 +209,15 @@ int rocshmem_amd_kv_attend(const rocshmem_amd_kv_cache_t *cache, int dtype, cons
   const int columns = columns_of(a.group, cache->head_dim);
   a.tiles = (a.group + 16 * columns - 1) / (16 * columns);
   const int64_t per_split = static_cast<int64_t>(n_seqs) * cache->kv_heads * a.tiles;
-  const size_t needed = part_bytes(rows, most_splits(per_split, max_len, 2 * a.cache.row_bytes), a.cache.head_dim);
+  a.splits = cut_of(per_split, max_len, 2 * a.cache.row_bytes, INT32_MAX);
+  const size_t needed = part_bytes(rows, a.splits.most, a.cache.head_dim);
   if (needed && (!workspace || !aligned_to(workspace, 16) || workspace_bytes < needed ||
                  !drv::local_ok(workspace, workspace_bytes)))
     return -1;
-  const Cut cut = cut_of(per_split, window > 0 && window < max_len ? window : max_len, 2 * a.cache.row_bytes);
-  a.split_units = cut.units;
-  a.splits = cut.splits;
+  if (window > 0 && window < max_len)  // no more splits than the workspace was asked for
+    a.splits = cut_of(per_split, window, 2 * a.cache.row_bytes, a.splits.most);
   a.part = static_cast<float *>(workspace);
-  a.part_stat = reinterpret_cast<F2 *>(a.part + rows * a.splits * a.cache.head_dim);
+  a.part_stat = reinterpret_cast<F2 *>(a.part + rows * a.splits.most * a.cache.head_dim);
   a.out_dtype = out_dtype;
   a.ctx = reinterpret_cast<const detail::Context *>(runtime::rt().driver_ctx_handle(my_pe).ctx_opaque);
   a.refused = runtime::rt().d_kv_refused;

@@ -27,6 +27,17 @@
 namespace rocshmem {
 namespace kv {
 
+// How a sequence's units of 16 tokens are split: n_big splits of `big`, then ones of
+// `small`; `most` over all for the longest sequence.
+struct Splits {
+  int big, n_big, small, most;
+  __host__ __device__ int begin(int i) const { return i < n_big ? i * big : n_big * big + (i - n_big) * small; }
+  __host__ __device__ int size(int i) const { return i < n_big ? big : small; }
+  __host__ __device__ int count(int units) const {  // how many have any of so many units
+    return units <= n_big * big ? (units + big - 1) / big : n_big + (units - n_big * big + small - 1) / small;
+  }
+};
+
 struct AttendArgs {
   Layout cache;
   const detail::Context *ctx;
@@ -42,7 +53,7 @@ struct AttendArgs {
   uint64_t table_row;
   int q_heads, group, tiles;  // query heads; how many share a cache head; work-groups that share them out
   int max_len, window, my_pe;
-  int split_units, splits;    // tokens of a split in units of 16, and how many at most
+  Splits splits;
   int out_dtype;
   bool own_pages;
   float scale, softcap;
@@ -146,8 +157,8 @@ __device__ __forceinline__ unsigned uniform(unsigned x) { return __builtin_amdgc
 
 // Wavefronts a SIMD is to hold: as many as the registers allow without spilling.
 constexpr int waves_of(int cache, int dim, int tiles) {
-  if (dim == 64) return tiles == 1 ? 4 : tiles == 4 ? 2 : 3;
-  if (dim == 128) return tiles > 1 ? 2 : cache == ROCSHMEM_AMD_E4M3 ? 4 : 3;
+  if (dim == 64) return tiles < 3 ? 3 : 2;
+  if (dim == 128) return tiles == 1 ? 3 : 2;
   return 2;
 }
 
@@ -183,6 +194,9 @@ void attend_kernel(AttendArgs a) {
     char keys[kAttendWaves][2][kUnitBytes];       // each wavefront's next step
     float out[kAttendWaves][16][kDim + 4];        // and at the end its sums
   } sh;
+  // Whether the registers hold a step's values as the products take them beside the
+  // next step's as they are loaded.
+  constexpr bool kEarly = kTiles < 4 && (kDim <= 128 || kNarrow);
   // Several tiles' queries would take the registers of another wavefront: they lie
   // in LDS, as the products' lanes hold them.
   constexpr bool kQueryInLds = kTiles > 1;
@@ -190,7 +204,10 @@ void attend_kernel(AttendArgs a) {
 
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int column = lane & 15, quad = lane >> 4;
-  const int b = blockIdx.y, split = blockIdx.z;
+  // Work-groups go round the XCDs in the order of their numbers.  A sequence's splits
+  // move on by one, or an XCD would get all of a long sequence where the cache heads
+  // and sequences fill whole rounds.
+  const int split = blockIdx.z, b = static_cast<int>((blockIdx.y + split) % gridDim.y);
   const uint32_t head = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles;
   const int head0 = head * a.group + tile * 16 * kTiles;
   const int heads_here = a.group - static_cast<int>(tile) * 16 * kTiles < 16 * kTiles
@@ -199,18 +216,19 @@ void attend_kernel(AttendArgs a) {
   // ---- the tokens: this wavefront's units of 16, a lane for each -----------------------
   // Without a window a unit's number does not depend on the sequence's length, and
   // its entry of the page table is asked for before the length is known.
-  const int per_wave = (a.split_units + 2 * kAttendWaves - 1) / (2 * kAttendWaves) * 2;  // at most 64
-  const int place = split * a.split_units + wave * per_wave + lane;
+  const int size = a.splits.size(split);
+  const int per_wave = (size + 2 * kAttendWaves - 1) / (2 * kAttendWaves) * 2;  // at most 64
+  const int place = a.splits.begin(split) + wave * per_wave + lane;
   const auto entry_of = [&](int unit) {
     const uint32_t index = quotient(static_cast<uint32_t>(unit), a.cache.by_page_units);
     return index < a.table_row ? static_cast<uint32_t>(a.page_table[b * a.table_row + index]) : ~0u;
   };
   uint32_t number = a.window > 0 ? 0u : entry_of(place);
   const Span span = span_of(a, b, blockIdx.x == 0 && split == 0 && threadIdx.x == 0);
-  const int first_unit = span.first_unit() + split * a.split_units;
-  const int end_unit = first_unit + a.split_units < span.end_unit() ? first_unit + a.split_units : span.end_unit();
+  const int first_unit = span.first_unit() + a.splits.begin(split);
+  const int end_unit = first_unit + size < span.end_unit() ? first_unit + size : span.end_unit();
   if (first_unit >= end_unit && split > 0) return;
-  const bool whole = span.end_unit() - span.first_unit() <= a.split_units;  // no other split has any
+  const bool whole = span.end_unit() - span.first_unit() <= a.splits.size(0);  // no other split has any
 
   unsigned page_lo, page_hi, unit_row;
   int unit_token, n_units;
@@ -416,7 +434,7 @@ void attend_kernel(AttendArgs a) {
     __builtin_amdgcn_s_waitcnt(kOnlyLds);
     __builtin_amdgcn_sched_barrier(0);
   };
-  const auto weigh = [&](int n, const Which &which, F4 (&s)[2], Weights &weights) {
+  const auto weigh = [&](int n, const Which &which, F4 (&s)[2], const unsigned (&scales)[2], Weights &weights) {
     if (a.softcap > 0.f) {
       // cap tanh(x), x = s / cap:  tanh(x) = 1 - 2 / (e^2x + 1)
       const float in_scale = 2.f * kLog2e / a.softcap;
@@ -455,7 +473,7 @@ void attend_kernel(AttendArgs a) {
         float p = __builtin_amdgcn_exp2f(s[u][r] - from);
         sum[n] += p;
         if constexpr (kNarrow) {
-          p *= two_to((value_scales[u] >> (8 * r)) & 0xff);
+          p *= two_to((scales[u] >> (8 * r)) & 0xff);
           if (which.cut) p = which.in[u][r] ? p : 0.f;
         }
         const typename PM::E high = static_cast<typename PM::E>(p);
@@ -495,48 +513,59 @@ void attend_kernel(AttendArgs a) {
       acc[n][c + 1] = PM::mul(__builtin_bit_cast(typename PM::V, odd), weights[part], acc[n][c + 1]);
     }
   };
-  // One step, tile by tile.  The next step's keys are asked for as soon as this
-  // one's have been read, its values as soon as this one's are used up.
+  // One step.  All scores first, and the values paired up: then nothing of what was
+  // loaded is wanted any more, and the next step's loads are on their way while
+  // this one's weights and sums are computed.
   const auto take = [&](int step, bool more) __attribute__((always_inline)) {
     const Which which = which_of(step);
-    F4 s[2];
-    Weights weights;
-    if constexpr (kTiles == 1) {
-      score(0, s);
+    if constexpr (kEarly) {
+      F4 s[kTiles][2];
+      U4 columns[kCols];
+      unsigned scales[2];
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) score(n, s[n]);
+      clear_values(which);
+#pragma unroll
+      for (int c = 0; c < kCols; c += 2) pair_up(c, columns[c], columns[c + 1]);
+      if constexpr (kNarrow) {
+        scales[0] = value_scales[0];
+        scales[1] = value_scales[1];
+      }
       if (more) {
         keys_are_read();
         load_keys(step + 1);
+        load_values(step + 1);
       }
-      weigh(0, which, s, weights);
-      clear_values(which);
-#pragma unroll
-      for (int c = 0; c < kCols; c += 2) {
-        U4 even, odd;
-        pair_up(c, even, odd);
-        add_pair(0, c, even, odd, weights);
-      }
-    } else {
-      // Paired up once for all tiles, as far as the registers reach.
-      constexpr bool kOnce = kTiles < 3;
-      U4 columns[kOnce ? kCols : 2];
 #pragma unroll
       for (int n = 0; n < kTiles; ++n) {
+        Weights weights;
+        weigh(n, which, s[n], scales, weights);
+#pragma unroll
+        for (int c = 0; c < kCols; c += 2) add_pair(n, c, columns[c], columns[c + 1], weights);
+      }
+    } else {
+      // Not enough registers for both: tile by tile, keys asked for when the last has
+      // scored, values at the end.
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) {
+        F4 s[2];
+        Weights weights;
         score(n, s);
         if (n == kTiles - 1 && more) {
           keys_are_read();
           load_keys(step + 1);
         }
-        weigh(n, which, s, weights);
+        weigh(n, which, s, value_scales, weights);
         if (n == 0) clear_values(which);
 #pragma unroll
         for (int c = 0; c < kCols; c += 2) {
-          const int at = kOnce ? c : 0;
-          if (!kOnce || n == 0) pair_up(c, columns[at], columns[at + 1]);
-          add_pair(n, c, columns[at], columns[at + 1], weights);
+          U4 even, odd;
+          pair_up(c, even, odd);
+          add_pair(n, c, even, odd, weights);
         }
       }
+      if (more) load_values(step + 1);
     }
-    if (more) load_values(step + 1);
   };
 
   const int steps = (n_units + 1) / 2;
@@ -600,7 +629,7 @@ void attend_kernel(AttendArgs a) {
         store_out(a, b, head0 + n * 16 + h, e, x);
         if (e == 0 && a.lse) a.lse[row] = (from + __builtin_amdgcn_logf(total)) * kLn2;
       } else {
-        const uint64_t at = row * a.splits + split;
+        const uint64_t at = row * a.splits.most + split;
         Eight<ROCSHMEM_AMD_FLOAT>::store(reinterpret_cast<char *>(a.part + at * d + e),
                                          Eight<ROCSHMEM_AMD_FLOAT>::round(x));
         if (e == 0) a.part_stat[at] = F2{from, total};
