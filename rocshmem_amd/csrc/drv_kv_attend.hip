@@ -20,12 +20,12 @@ constexpr int kMostTokens = 1 << 25;  // of a sequence: 2^15 of the smallest spl
 // Joins a sequence's splits: out = sum_i 2^(t_i - t) o_i / sum_i 2^(t_i - t) l_i over the
 // splits that have tokens, t the largest t_i.  One work-group per sequence and
 // query head: kLanes lanes along the row, four elements each, and the splits dealt
-// out to the 256 / kLanes groups, four of a group's on their way at once.  Each
+// out to the kThreads / kLanes groups, four of a group's on their way at once.  Each
 // group keeps its own largest t_i as it goes, and the first four are asked for
 // before the length, which only says how many of them count.
-template <int kLanes>
-__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
-  constexpr int kGroups = 256 / kLanes, kAhead = 4;
+template <int kLanes, int kThreads>
+__global__ __launch_bounds__(kThreads) void attend_join_kernel(AttendArgs a) {
+  constexpr int kGroups = kThreads / kLanes, kAhead = 4;
   const int b = blockIdx.y, h = blockIdx.x, lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   const uint64_t row = static_cast<uint64_t>(b) * a.q_heads + h;
   const F2 *stat = a.part_stat + row * a.splits.most;
@@ -146,13 +146,21 @@ static void launch_attend(const AttendArgs &a, int n_seqs, hipStream_t s) {
     launch_columns<kQ, kC, 256>(a, n_seqs, columns, s);
   DRV_CHECK_HIP(hipGetLastError());
   if (a.splits.most > 1) {
-    const dim3 rows(a.q_heads, n_seqs);
+    // A wavefront for a row where there are few splits, four otherwise.
+    const auto join = [&](auto lanes) {
+      constexpr int kLanes = decltype(lanes)::value;
+      const dim3 rows(a.q_heads, n_seqs);
+      if (a.splits.most <= 4 * 64 / kLanes)
+        hipLaunchKernelGGL((attend_join_kernel<kLanes, 64>), rows, dim3(64), 0, s, a);
+      else
+        hipLaunchKernelGGL((attend_join_kernel<kLanes, 256>), rows, dim3(256), 0, s, a);
+    };
     if (a.cache.head_dim <= 64)
-      hipLaunchKernelGGL(attend_join_kernel<16>, rows, dim3(256), 0, s, a);
+      join(std::integral_constant<int, 16>{});
     else if (a.cache.head_dim <= 128)
-      hipLaunchKernelGGL(attend_join_kernel<32>, rows, dim3(256), 0, s, a);
+      join(std::integral_constant<int, 32>{});
     else
-      hipLaunchKernelGGL(attend_join_kernel<64>, rows, dim3(256), 0, s, a);
+      join(std::integral_constant<int, 64>{});
     DRV_CHECK_HIP(hipGetLastError());
   }
 }

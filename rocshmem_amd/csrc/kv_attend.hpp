@@ -156,9 +156,9 @@ __device__ __forceinline__ float sum_of_column(float x) {
 __device__ __forceinline__ unsigned uniform(unsigned x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // Wavefronts a SIMD is to hold: as many as the registers allow without spilling.
-constexpr int waves_of(int cache, int dim, int tiles) {
+constexpr int waves_of(int dim, int tiles) {
   if (dim == 64) return tiles < 3 ? 3 : 2;
-  if (dim == 128) return tiles == 1 ? 3 : 2;
+  if (dim == 128) return tiles == 1 ? 3 : tiles == 4 ? 1 : 2;
   return 2;
 }
 
@@ -169,7 +169,7 @@ constexpr int waves_of(int cache, int dim, int tiles) {
 // kQ: the activations' type, kC: the cache's; kDim: head_dim rounded up to 64, 128
 // or 256; kWhole: one split.
 template <int kQ, int kC, int kDim, int kTiles, bool kWhole>
-__global__ __launch_bounds__(64 * (kWhole ? kWholeWaves : kSplitWaves), kWhole ? 2 : waves_of(kC, kDim, kTiles))
+__global__ __launch_bounds__(64 * (kWhole ? kWholeWaves : kSplitWaves), kWhole ? 2 : waves_of(kDim, kTiles))
 void attend_kernel(AttendArgs a) {
   constexpr int kAttendWaves = kWhole ? kWholeWaves : kSplitWaves;
   constexpr bool kNarrow = kC == ROCSHMEM_AMD_E4M3;
@@ -196,7 +196,7 @@ void attend_kernel(AttendArgs a) {
   } sh;
   // Whether the registers hold a step's values as the products take them beside the
   // next step's as they are loaded.
-  constexpr bool kEarly = kTiles < 4 && (kDim <= 128 || kNarrow);
+  constexpr bool kEarly = kDim <= 128 || kNarrow;
   // Several tiles' queries would take the registers of another wavefront: they lie
   // in LDS, as the products' lanes hold them.
   constexpr bool kQueryInLds = kTiles > 1;
