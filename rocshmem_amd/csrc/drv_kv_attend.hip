@@ -92,7 +92,7 @@ __global__ __launch_bounds__(kThreads) void attend_join_kernel(AttendArgs a) {
 // How a call is cut: at most `limit` splits for the longest sequence.
 static Splits cut_of(int64_t work_groups_per_split, int64_t max_tokens, int64_t token_bytes, int limit) {
   const int64_t units = (max_tokens + 15) / 16 + 1;  // a window may start inside a unit
-  if (units <= kWholeUnits) return Splits{static_cast<int>(units), 1, 1, 1};
+  if (left_whole(units, work_groups_per_split)) return Splits{static_cast<int>(units), 1, 1, 1};
   const auto whole_steps = [](int64_t n) { return (n + 2 * kSplitWaves - 1) / (2 * kSplitWaves) * (2 * kSplitWaves); };
   const int64_t wanted = (kWantedWorkGroups + work_groups_per_split - 1) / work_groups_per_split;
   const int64_t most = kMostSplitBytes / (16 * token_bytes) < kMostUnits ? kMostSplitBytes / (16 * token_bytes) : kMostUnits;
