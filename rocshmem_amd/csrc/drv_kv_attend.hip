@@ -4,18 +4,8 @@
 namespace rocshmem {
 namespace kv {
 
-// Splits are cut for about this many work-groups over all (two for each CU), and of at
-// most so many bytes of the cache; the second half of the longest sequence into
-// splits a third as long.  Work-groups start in the order of their numbers, so the
-// short ones fill the gaps at the end, where a CU with one long split more than the
-// others would be waited for (a CU takes little more than its share of the memory's
-// rate, so a split too many on it is not made up for).  Measured, us, with equal
-// splits / with a half in thirds: 64 sequences to 4096 bf16 93.9 / 90.0, 48 heads on one
-// 52.4 / 45.3, 16 sequences with own heads 27.3 / 25.8, 2 to 131072 e4m3 69.2 / 68.8;
-// 1024 work-groups instead of 512: 90, 58, 26, 73; splits of 2 MiB: 105 for the first.
-constexpr int64_t kWantedWorkGroups = 512, kMostSplitBytes = 1 << 20;
-constexpr int64_t kLeastUnits = 16;  // of a short split: two steps of its wavefronts
-constexpr int kMostTokens = 1 << 25;  // of a sequence: 2^15 of the smallest splits that kMostSplitBytes gives
+constexpr int kMostTokens = 1 << 25;  // of a sequence
+constexpr int64_t kWantedWorkGroups = 512;  // two for each CU
 
 // Joins a sequence's splits: out = sum_i 2^(t_i - t) o_i / sum_i 2^(t_i - t) l_i over the
 // splits that have tokens, t the largest t_i.  One work-group per sequence and
@@ -28,9 +18,9 @@ __global__ __launch_bounds__(kThreads) void attend_join_kernel(AttendArgs a) {
   constexpr int kGroups = kThreads / kLanes, kAhead = 4;
   const int b = blockIdx.y, h = blockIdx.x, lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   const uint64_t row = static_cast<uint64_t>(b) * a.q_heads + h;
-  const F2 *stat = a.part_stat + row * a.splits.most;
+  const F2 *stat = a.part_stat + row * a.most_splits;
   const uint32_t d = a.cache.head_dim;
-  const float *part = a.part + row * a.splits.most * d + (lane * 4u < d ? lane * 4 : 0);
+  const float *part = a.part + row * a.most_splits * d + (lane * 4u < d ? lane * 4 : 0);
   __shared__ F2 sh_stat[kGroups];
   __shared__ F4 sh_out[kGroups][kLanes];
   F2 s[kAhead];
@@ -38,7 +28,7 @@ __global__ __launch_bounds__(kThreads) void attend_join_kernel(AttendArgs a) {
   const auto load = [&](int i0) {
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      const int i = i0 + k * kGroups, at = i < a.splits.most ? i : 0;
+      const int i = i0 + k * kGroups, at = i < a.most_splits ? i : 0;
       s[k] = stat[at];
       o[k] = *reinterpret_cast<const F4 *>(part + static_cast<uint64_t>(at) * d);
     }
@@ -46,7 +36,7 @@ __global__ __launch_bounds__(kThreads) void attend_join_kernel(AttendArgs a) {
   load(group);
   const Span span = span_of(a, b, false);
   const int units = span.end_unit() - span.first_unit();
-  const int n = a.splits.count(units);
+  const int n = splits_here(a, units).count(units);
   if (n <= 1) return;  // its only split has written the result
   float top = -INFINITY, total = 0.f;
   F4 x{0.f, 0.f, 0.f, 0.f};
@@ -89,26 +79,18 @@ __global__ __launch_bounds__(kThreads) void attend_join_kernel(AttendArgs a) {
   if (a.lse && threadIdx.x == 0) a.lse[row] = (top + __builtin_amdgcn_logf(total)) * kLn2;
 }
 
-// How a call is cut: at most `limit` splits for the longest sequence.
-static Splits cut_of(int64_t work_groups_per_split, int64_t max_tokens, int64_t token_bytes, int limit) {
-  const int64_t units = (max_tokens + 15) / 16 + 1;  // a window may start inside a unit
-  if (left_whole(units, work_groups_per_split)) return Splits{static_cast<int>(units), 1, 1, 1};
-  const auto whole_steps = [](int64_t n) { return (n + 2 * kSplitWaves - 1) / (2 * kSplitWaves) * (2 * kSplitWaves); };
-  const int64_t wanted = (kWantedWorkGroups + work_groups_per_split - 1) / work_groups_per_split;
-  const int64_t most = kMostSplitBytes / (16 * token_bytes) < kMostUnits ? kMostSplitBytes / (16 * token_bytes) : kMostUnits;
-  int64_t big = (units + wanted - 1) / wanted;
-  if (big > most) big = most;
-  if (big >= units) big = (units + 1) / 2;
-  big = whole_steps(big);
-  int64_t small = whole_steps(big / 3 > kLeastUnits ? big / 3 : kLeastUnits);
-  for (;;) {
-    const int64_t n_big = units / 2 / big > 1 ? units / 2 / big : 1;
-    Splits s{static_cast<int>(big), static_cast<int>(n_big), static_cast<int>(small), 0};
-    s.most = s.count(static_cast<int>(units));
-    if (s.most <= limit || small >= kMostUnits) return s;
-    big = 2 * big < kMostUnits ? 2 * big : kMostUnits;
-    small = 2 * small < kMostUnits ? 2 * small : kMostUnits;
-  }
+// How a call is cut.  most_splits 1: sequences are not split.
+struct Cut {
+  Splits splits;  // of the bound
+  int units, wanted, most_splits;
+};
+static Cut cut_of(int64_t work_groups_per_split, int64_t max_tokens, bool window) {
+  // (a window may start inside a unit)
+  const int units = static_cast<int>((max_tokens + 15) / 16) + (window || max_tokens == 0 ? 1 : 0);
+  if (left_whole(units, work_groups_per_split)) return Cut{Splits{units, 1, 1}, units, 1, 1};
+  const int64_t each = (kWantedWorkGroups + work_groups_per_split - 1) / work_groups_per_split;
+  const int wanted = each > 2 ? static_cast<int>(each) : 2;
+  return Cut{splits_of(units, wanted), units, wanted, static_cast<int>(most_splits(units, wanted))};
 }
 static int columns_of(int group, int head_dim) {  // tiles of 16 query heads that one work-group takes
   const int tiles = (group + 15) / 16, most = head_dim > 128 ? 1 : 4;
@@ -120,8 +102,8 @@ static size_t part_bytes(size_t rows, size_t splits, size_t head_dim) {
 
 template <int kQ, int kC, int kDim, int kTiles>
 static void launch_one(const AttendArgs &a, int n_seqs, hipStream_t s) {
-  const dim3 grid(a.cache.kv_heads * a.tiles, n_seqs, a.splits.most);
-  if (a.splits.most == 1)
+  const dim3 grid(a.cache.kv_heads * a.tiles, n_seqs, a.most_splits);
+  if (a.most_splits == 1)
     hipLaunchKernelGGL((attend_kernel<kQ, kC, kDim, kTiles, true>), grid, dim3(64 * kWholeWaves), 0, s, a);
   else
     hipLaunchKernelGGL((attend_kernel<kQ, kC, kDim, kTiles, false>), grid, dim3(64 * kSplitWaves), 0, s, a);
@@ -145,12 +127,12 @@ static void launch_attend(const AttendArgs &a, int n_seqs, hipStream_t s) {
   else
     launch_columns<kQ, kC, 256>(a, n_seqs, columns, s);
   DRV_CHECK_HIP(hipGetLastError());
-  if (a.splits.most > 1) {
+  if (a.most_splits > 1) {
     // A wavefront for a row where there are few splits, four otherwise.
     const auto join = [&](auto lanes) {
       constexpr int kLanes = decltype(lanes)::value;
       const dim3 rows(a.q_heads, n_seqs);
-      if (a.splits.most <= 4 * 64 / kLanes)
+      if (a.most_splits <= 4 * 64 / kLanes)
         hipLaunchKernelGGL((attend_join_kernel<kLanes, 64>), rows, dim3(64), 0, s, a);
       else
         hipLaunchKernelGGL((attend_join_kernel<kLanes, 256>), rows, dim3(256), 0, s, a);
@@ -180,7 +162,7 @@ size_t rocshmem_amd_kv_attend_bytes(const rocshmem_amd_kv_cache_t *cache, int n_
   const int group = q_heads / cache->kv_heads, columns = columns_of(group, cache->head_dim);
   const int64_t tiles = (group + 16 * columns - 1) / (16 * columns);
   return part_bytes(static_cast<size_t>(n_seqs) * q_heads,
-                    cut_of(n_seqs * tiles * cache->kv_heads, max_len, 2 * c.row_bytes, INT32_MAX).most, c.head_dim);
+                    cut_of(n_seqs * tiles * cache->kv_heads, max_len, true).most_splits, c.head_dim);
 }
 
 int rocshmem_amd_kv_attend(const rocshmem_amd_kv_cache_t *cache, int dtype, const void *q, size_t q_row,
@@ -217,15 +199,18 @@ int rocshmem_amd_kv_attend(const rocshmem_amd_kv_cache_t *cache, int dtype, cons
   const int columns = columns_of(a.group, cache->head_dim);
   a.tiles = (a.group + 16 * columns - 1) / (16 * columns);
   const int64_t per_split = static_cast<int64_t>(n_seqs) * cache->kv_heads * a.tiles;
-  a.splits = cut_of(per_split, max_len, 2 * a.cache.row_bytes, INT32_MAX);
-  const size_t needed = part_bytes(rows, a.splits.most, a.cache.head_dim);
+  const size_t needed = part_bytes(rows, cut_of(per_split, max_len, true).most_splits, a.cache.head_dim);
   if (needed && (!workspace || !aligned_to(workspace, 16) || workspace_bytes < needed ||
                  !drv::local_ok(workspace, workspace_bytes)))
     return -1;
-  if (window > 0 && window < max_len)  // no more splits than the workspace was asked for
-    a.splits = cut_of(per_split, window, 2 * a.cache.row_bytes, a.splits.most);
+  // (a window or none, no more splits than that)
+  const Cut cut = cut_of(per_split, window > 0 && window < max_len ? window : max_len, window > 0);
+  a.bound_splits = cut.splits;
+  a.bound_units = cut.units;
+  a.wanted = cut.wanted;
+  a.most_splits = cut.most_splits;
   a.part = static_cast<float *>(workspace);
-  a.part_stat = reinterpret_cast<F2 *>(a.part + rows * a.splits.most * a.cache.head_dim);
+  a.part_stat = reinterpret_cast<F2 *>(a.part + rows * a.most_splits * a.cache.head_dim);
   a.out_dtype = out_dtype;
   a.ctx = reinterpret_cast<const detail::Context *>(runtime::rt().driver_ctx_handle(my_pe).ctx_opaque);
   a.refused = runtime::rt().d_kv_refused;
@@ -237,6 +222,7 @@ int rocshmem_amd_kv_attend(const rocshmem_amd_kv_cache_t *cache, int dtype, cons
   a.q_row = q_row;
   a.out_row = out_row;
   a.table_row = table_row;
+  a.n_seqs = n_seqs;
   a.q_heads = q_heads;
   a.max_len = max_len;
   a.window = window;

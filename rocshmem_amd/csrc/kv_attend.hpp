@@ -27,17 +27,6 @@
 namespace rocshmem {
 namespace kv {
 
-// How a sequence's units of 16 tokens are split: n_big splits of `big`, then ones of
-// `small`; `most` over all for the longest sequence.
-struct Splits {
-  int big, n_big, small, most;
-  __host__ __device__ int begin(int i) const { return i < n_big ? i * big : n_big * big + (i - n_big) * small; }
-  __host__ __device__ int size(int i) const { return i < n_big ? big : small; }
-  __host__ __device__ int count(int units) const {  // how many have any of so many units
-    return units <= n_big * big ? (units + big - 1) / big : n_big + (units - n_big * big + small - 1) / small;
-  }
-};
-
 struct AttendArgs {
   Layout cache;
   const detail::Context *ctx;
@@ -51,9 +40,13 @@ struct AttendArgs {
   F2 *part_stat;      // [sequence][query head][split]: exponent the sums are taken from, and sum
   uint64_t q_row, out_row;  // elements between sequences
   uint64_t table_row;
+  int n_seqs;
   int q_heads, group, tiles;  // query heads; how many share a cache head; work-groups that share them out
   int max_len, window, my_pe;
-  Splits splits;
+  // else: how the bound would be split, of how many units, and what is asked of
+  // splits_of where the sequences are shorter; how many splits one can have at most
+  Splits bound_splits;
+  int bound_units, wanted, most_splits;
   int out_dtype;
   bool own_pages;
   float scale, softcap;
@@ -105,17 +98,6 @@ __device__ __forceinline__ void stream_to_lds(GlobalBytes from, uint32_t offset,
                                    (__attribute__((address_space(3))) void *)to, 16, 0, kNonTemporal);
 }
 
-// Short sequences take a work-group of eight wavefronts each and no second kernel;
-// longer ones are split over work-groups of four.
-constexpr int kSplitWaves = 4, kWholeWaves = 8;
-constexpr int kMostUnits = 64 * kSplitWaves;  // of a split: a lane for each of a wavefront's
-// Not split are sequences of at most 48 units, three steps of a wavefront, or 72 where
-// that fills half the GPU.  Measured, us, whole / split: 1 sequence of 600 tokens and 8
-// cache heads in bf16 8.7 / 11.6, of 1000 13.7 / 11.6, 8 of 1000 14.4 / 12.1, 32 of 1000
-// 17.4 / 19.7, 16 of 2000 26.0 / 20.4.
-__host__ __device__ constexpr bool left_whole(int64_t units, int64_t work_groups) {
-  return units <= (work_groups >= 128 ? 72 : 48);
-}
 // The matrix product of a type, and pairs of values rounded to it.
 template <int kType>
 struct Mma;
@@ -159,9 +141,30 @@ __device__ __forceinline__ float sum_of_column(float x) {
   r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+// The splits of a sequence of `own` units: the same for all of a call, up to a number
+// of sequences that a wavefront can look at.
+__device__ __forceinline__ Splits splits_here(const AttendArgs &a, int own) {
+  const int near = a.bound_units - a.bound_units / 4;
+  int most = own;
+  if (a.n_seqs <= kMostLooked) {
+    for (int i = threadIdx.x & 63; i < a.n_seqs; i += 64) {
+      const Span s = span_of(a, i, false);
+      const int units = s.end_unit() - s.first_unit();
+      most = units > most ? units : most;
+    }
+    if (!__any(most >= near))
+      for (int hop = 32; hop; hop /= 2) {
+        const int other = __shfl_xor(most, hop);
+        most = other > most ? other : most;
+      }
+  }
+  if (__any(most >= near)) return a.bound_splits;
+  return splits_of(__builtin_amdgcn_readfirstlane(most), a.wanted);
+}
 __device__ __forceinline__ unsigned uniform(unsigned x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// Wavefronts a SIMD is to hold: as many as the registers allow without spilling.
+// Wavefronts a SIMD is to hold: as many as the registers allow without spilling in
+// the loop (a work-group of eight is two, whose four tiles at 128 spill 84 to 96 bytes).
 constexpr int waves_of(int dim, int tiles) {
   if (dim == 64) return tiles < 3 ? 3 : 2;
   if (dim == 128) return tiles == 1 ? 3 : tiles == 4 ? 1 : 2;
@@ -219,34 +222,52 @@ void attend_kernel(AttendArgs a) {
   const int heads_here = a.group - static_cast<int>(tile) * 16 * kTiles < 16 * kTiles
                              ? a.group - static_cast<int>(tile) * 16 * kTiles : 16 * kTiles;
 
-  // ---- the tokens: this wavefront's units of 16, a lane for each -----------------------
-  // Without a window a unit's number does not depend on the sequence's length, and
-  // its entry of the page table is asked for before the length is known.
-  const int size = a.splits.size(split);
-  const int per_wave = (size + 2 * kAttendWaves - 1) / (2 * kAttendWaves) * 2;  // at most 64
-  const int place = a.splits.begin(split) + wave * per_wave + lane;
+  // ---- the tokens: units of 16, a lane for each of this wavefront's ---------------------
   const auto entry_of = [&](int unit) {
     const uint32_t index = quotient(static_cast<uint32_t>(unit), a.cache.by_page_units);
     return index < a.table_row ? static_cast<uint32_t>(a.page_table[b * a.table_row + index]) : ~0u;
   };
-  uint32_t number = a.window > 0 ? 0u : entry_of(place);
+  // A wavefront's units: runs of at most 64, one after the other, from `from` on.
+  struct Runs {
+    int from, size, each;  // of all wavefronts over all; of this one in a run
+  };
+  const auto runs_of = [&](const Splits &splits) {
+    const int full = splits.size(split), runs = (full + 64 * kAttendWaves - 1) / (64 * kAttendWaves);
+    const int run = runs > 1 ? (full + runs - 1) / runs : full;
+    return Runs{splits.begin(split), full, (run + 2 * kAttendWaves - 1) / (2 * kAttendWaves) * 2};
+  };
+  // Without a window, where the splits are the bound's, a unit's number does not
+  // depend on any length, and its entry of the page table is asked for before they
+  // are known.
+  Runs runs = runs_of(a.bound_splits);
+  const uint32_t first_number = a.window > 0 ? 0u : entry_of(runs.from + wave * runs.each + lane);
+  bool known = a.window == 0;
   const Span span = span_of(a, b, blockIdx.x == 0 && split == 0 && threadIdx.x == 0);
-  const int first_unit = span.first_unit() + a.splits.begin(split);
-  const int end_unit = first_unit + size < span.end_unit() ? first_unit + size : span.end_unit();
-  if (first_unit >= end_unit && split > 0) return;
-  const bool whole = span.end_unit() - span.first_unit() <= a.splits.size(0);  // no other split has any
+  const int units = span.end_unit() - span.first_unit();
+  bool whole = true;  // no other split has any
+  if constexpr (!kWhole) {
+    const Splits splits = splits_here(a, units);
+    const Runs here = runs_of(splits);
+    known = known && here.from == runs.from && here.each == runs.each;
+    runs = here;
+    if (runs.from >= units && split > 0) return;
+    whole = splits.count(units) <= 1;
+  }
+  const int end = runs.from + runs.size < units ? runs.from + runs.size : units;
 
   unsigned page_lo, page_hi, unit_row;
   int unit_token, n_units;
-  {
-    const int unit = span.first_unit() + place;
-    bool there = lane < per_wave && unit < end_unit;
-    if (a.window > 0 && there) number = entry_of(unit);
+  // The pages of the units [first, first + count), at most 64, counted from the
+  // sequence's first.
+  const auto look_up = [&](int first, int count, bool known) __attribute__((always_inline)) {
+    const int unit = span.first_unit() + first + lane;
+    bool there = lane < count;
     uint64_t page = 0;
     uint32_t at = 0;
     if (there) {
       const uint32_t index = quotient(static_cast<uint32_t>(unit), a.cache.by_page_units);
       at = static_cast<uint32_t>(unit) * 16 - index * a.cache.page_tokens;
+      const uint32_t number = known ? first_number : entry_of(unit);
       if (number >= a.cache.n_pages) {
         there = false;
         if (blockIdx.x == 0 && (at == 0 || unit == span.first_unit())) count_refused(a.refused);
@@ -273,7 +294,7 @@ void attend_kernel(AttendArgs a) {
       unit_row = __builtin_amdgcn_ds_permute(to, unit_row);
       unit_token = __builtin_amdgcn_ds_permute(to, unit_token);
     }
-  }
+  };
 
   // ---- the query, and where the lane's loads are from a unit's first row -----------
   // A unit's keys are one run of 16 rows.  They are fetched as they lie, 1 KiB at a
@@ -374,7 +395,8 @@ void attend_kernel(AttendArgs a) {
     }
   };
 
-  constexpr int kOnlyLds = 0xc07f;  // s_waitcnt lgkmcnt(0), leaving loads on their way
+  constexpr int kOnlyLds = 0xc07f;    // s_waitcnt lgkmcnt(0), leaving loads on their way
+  constexpr int kOnlyLoads = 0x0f70;  // s_waitcnt vmcnt(0)
   typedef typename PM::V Weights[2];  // rounded, and what the rounding left
   struct Which {                      // of a step's tokens take part
     bool cut, in[2][4];
@@ -433,6 +455,11 @@ void attend_kernel(AttendArgs a) {
         if constexpr (kNarrow) up *= two_to((key_scales[u] >> (8 * r)) & 0xff);
         s[u][r] *= up;
       }
+  };
+  // What this step multiplies has arrived: keys in LDS, values in registers.
+  const auto loads_are_here = [&] {
+    __builtin_amdgcn_s_waitcnt(kOnlyLoads);
+    __builtin_amdgcn_sched_barrier(0);
   };
   // The keys in LDS have been read, and not only asked for, before the next ones
   // may be fetched over them.
@@ -524,6 +551,7 @@ void attend_kernel(AttendArgs a) {
   // this one's weights and sums are computed.
   const auto take = [&](int step, bool more) __attribute__((always_inline)) {
     const Which which = which_of(step);
+    loads_are_here();
     if constexpr (kEarly) {
       F4 s[kTiles][2];
       U4 columns[kCols];
@@ -574,18 +602,33 @@ void attend_kernel(AttendArgs a) {
     }
   };
 
-  const int steps = (n_units + 1) / 2;
-  if (steps > 0) {
-    load_keys(0);
-    load_values(0);
-  }
-  if constexpr (kQueryInLds) __syncthreads();
-  if (steps > 0) {
+  const auto begin_steps = [&](int first, bool known) __attribute__((always_inline)) {
+    const int left = end - first;
+    look_up(first, left < runs.each ? left : runs.each, known);
+    if (n_units > 0) {
+      load_keys(0);
+      load_values(0);
+    }
+  };
+  const auto take_steps = [&]() __attribute__((always_inline)) {
     // The last step stands by itself, so that no wait has to allow for loads that
     // were not made.
+    const int steps = (n_units + 1) / 2;
     int step = 0;
     for (; step + 1 < steps; ++step) take(step, true);
-    take(step, false);
+    if (steps > 0) take(step, false);
+  };
+  if constexpr (kWhole) {
+    begin_steps(wave * runs.each, known);
+    if constexpr (kQueryInLds) __syncthreads();
+    take_steps();
+  } else {
+    if constexpr (kQueryInLds) __syncthreads();
+    for (int first = runs.from; first < end; first += runs.each * kAttendWaves) {
+      begin_steps(first + wave * runs.each, known && first == runs.from);
+      take_steps();
+      keys_are_read();
+    }
   }
 
   // ---- the wavefronts' sums joined -----------------------------------------------
@@ -635,7 +678,7 @@ void attend_kernel(AttendArgs a) {
         store_out(a, b, head0 + n * 16 + h, e, x);
         if (e == 0 && a.lse) a.lse[row] = (from + __builtin_amdgcn_logf(total)) * kLn2;
       } else {
-        const uint64_t at = row * a.splits.most + split;
+        const uint64_t at = row * a.most_splits + split;
         Eight<ROCSHMEM_AMD_FLOAT>::store(reinterpret_cast<char *>(a.part + at * d + e),
                                          Eight<ROCSHMEM_AMD_FLOAT>::round(x));
         if (e == 0) a.part_stat[at] = F2{from, total};

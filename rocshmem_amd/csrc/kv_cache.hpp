@@ -125,6 +125,63 @@ inline bool fill_layout(int dtype, int page_tokens, int kv_heads, int head_dim, 
   return true;
 }
 
+// ---- how attention's work is cut ---------------------------------------------------
+
+// How a sequence's units of 16 tokens are split over work-groups: n_big splits of
+// `big`, the rest into ones of `small`.
+struct Splits {
+  int big, n_big, small;
+  __host__ __device__ int begin(int i) const { return i < n_big ? i * big : n_big * big + (i - n_big) * small; }
+  __host__ __device__ int size(int i) const { return i < n_big ? big : small; }
+  __host__ __device__ int count(int units) const {  // how many have any of so many units
+    return units <= n_big * big ? (units + big - 1) / big : n_big + (units - n_big * big + small - 1) / small;
+  }
+};
+
+// Short sequences take a work-group of eight wavefronts each and no second kernel;
+// longer ones are split over work-groups of four.
+constexpr int kSplitWaves = 4, kWholeWaves = 8;
+// How sequences are split: the first half of the longest as for `wanted` equal
+// splits, the second half into splits a third as long (whole steps of the
+// wavefronts, no shorter than two), and all sequences alike.  Work-groups start in
+// the order of their numbers, so the short splits fill the gaps at the end, where a
+// CU with one long split more than the others would be waited for (a CU takes little
+// more than its share of the memory's rate, so a split too many on it is not made
+// up for).  Measured, us, in equal splits / with a half in thirds: 64 sequences to
+// 4096 tokens in bf16 93.9 / 90.0, 48 heads on one 52.4 / 45.3, 16 sequences with own
+// heads 27.3 / 25.8, 2 to 131072 in e4m3 69.2 / 68.8.
+//
+// The longest is the longest of the call as a wavefront finds it, not the bound that
+// a captured call has to give: 64 sequences of 400 tokens and 8 cache heads under a
+// bound of 131072 took 68 us split by the bound, 18 so.  Only where it is near the
+// bound is the bound taken, whose splits' places are known beforehand (looking costs
+// such a call about 1 us).
+constexpr int kMostLooked = 1024;       // sequences
+constexpr int kStep = 2 * kSplitWaves;  // units of a step of all wavefronts
+__host__ __device__ inline Splits splits_of(int units, int wanted) {
+  if (units <= 6 * kStep) return Splits{6 * kStep, 1, 2 * kStep};  // one
+  int big = (units + wanted - 1) / wanted, small = 2 * kStep;
+  big = big > 3 * kStep ? (big + kStep - 1) / kStep * kStep : 3 * kStep;
+  if (big / 3 > small) small = (big / 3 + kStep - 1) / kStep * kStep;
+  const int n_big = units / 2 / big;
+  return Splits{big, n_big > 1 ? n_big : 1, small};
+}
+// The most splits of a sequence of at most so many units.  With x = units / big <=
+// wanted there are floor(x / 2) big ones (one at least) and at most ceil(3 (x - floor(x / 2)))
+// small ones, 2 wanted + 2 together (four for wanted = 2, where big is half); and no
+// small one is shorter than two steps.
+inline int64_t most_splits(int64_t units, int64_t wanted) {
+  const int64_t by_number = wanted == 2 ? 4 : 2 * wanted + 2, by_length = units / (2 * kStep) + 2;
+  return by_number < by_length ? by_number : by_length;
+}
+// Not split are sequences of at most 48 units, three steps of a wavefront, or 72 where
+// that fills half the GPU.  Measured, us, whole / split: 1 sequence of 600 tokens and 8
+// cache heads in bf16 8.7 / 11.6, of 1000 13.7 / 11.6, 8 of 1000 14.4 / 12.1, 32 of 1000
+// 17.4 / 19.7, 16 of 2000 26.0 / 20.4.
+__host__ __device__ constexpr bool left_whole(int64_t units, int64_t work_groups) {
+  return units <= (work_groups >= 128 ? 72 : 48);
+}
+
 }  // namespace kv
 }  // namespace rocshmem
 
