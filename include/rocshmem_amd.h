@@ -690,7 +690,8 @@ int rocshmem_amd_ctx_cycle(rocshmem_amd_team_t team, int n_wgs, int wg_size, int
  * current one.  As with putmem, rows put to another PE may be read there after
  * a barrier (or stream order, where all PEs share the stream).  Slots, page
  * numbers and lengths are read by the kernels; what is out of range is left
- * out, never followed, and counted (rocshmem_amd_kv_refused). */
+ * out, never followed, and counted (rocshmem_amd_kv_refused).  What a call
+ * writes overlaps nothing that it reads, nor its other outputs. */
 typedef struct rocshmem_amd_kv_cache {
   void *pages;      /* symmetric: pages_per_pe * page_bytes per PE, 16-byte aligned */
   int dtype;        /* ROCSHMEM_AMD_BF16, _HALF or _E4M3 */
@@ -747,9 +748,12 @@ int rocshmem_amd_kv_get(const rocshmem_amd_kv_cache_t *cache, int dtype, void *k
  * q: n_seqs x q_heads x head_dim of `dtype` (the cache's, or BF16 or HALF for an
  * E4M3 cache), sequence b's at q + b * q_row elements.  out: the same shape in
  * out_dtype (`dtype`, or FLOAT for partial results), rows out_row elements
- * apart (at least q_heads * head_dim).  max_len: at most 2^25.  lse: n_seqs x q_heads floats, or NULL.
- * A length above max_len, or above what table_row pages hold, counts as that
- * (and is counted as refused); a negative one as 0 (the same).
+ * apart (at least q_heads * head_dim).  lse: n_seqs x q_heads floats, or NULL.
+ * softcap: 0, or at least 2^-100.  max_len: at most 2^25; a bound, so that a
+ * captured call serves sequences that grow (the work is cut by the lengths that
+ * a call finds, a generous bound costs a few us).  A length above max_len, or
+ * above what table_row pages hold, counts as that (and is counted as refused);
+ * a negative one as 0 (the same).
  * workspace: device memory of at least rocshmem_amd_kv_attend_bytes bytes,
  * 16-byte aligned, whose content does not matter; calls that may overlap in
  * time need one each. */
@@ -773,8 +777,9 @@ int rocshmem_amd_kv_attend(const rocshmem_amd_kv_cache_t *cache, int dtype, cons
  * goes to my_pe's out (out_dtype: BF16, HALF or FLOAT) and lse (may be NULL).  A
  * member whose lse_i is -infinity takes no part, whatever its o_i holds; with
  * none left out is 0 and lse -infinity.  One-sided, like a get: call it once
- * the members' results are complete.  The members are folded in ascending
- * order.  head_dim: a multiple of 8; partial 16-byte aligned. */
+ * the members' results are complete; out and lse may not overlap my_pe's.  The
+ * members are folded in ascending order.  head_dim: a multiple of 8; partial
+ * 16-byte aligned. */
 int rocshmem_amd_kv_join(int dtype, const void *partial, const float *partial_lse, size_t n_rows,
                          int head_dim, int out_dtype, void *out, float *lse, int PE_start,
                          int logPE_stride, int PE_size, int my_pe, rocshmem_amd_stream_t stream);

@@ -349,6 +349,10 @@ int rocshmem_amd_kv_join(int dtype, const void *partial, const float *partial_ls
     return -1;
   if (!out || !aligned_to(out, out_es) || !drv::local_ok(out, out_bytes)) return -1;
   if (!aligned_to(lse, 4) || (lse && !drv::local_ok(lse, lse_bytes))) return -1;
+  // Nothing that is still to be read may be written over.
+  if (overlap(out, out_bytes, partial, bytes) || overlap(out, out_bytes, partial_lse, lse_bytes) ||
+      overlap(lse, lse ? lse_bytes : 0, partial, bytes) || overlap(lse, lse ? lse_bytes : 0, partial_lse, lse_bytes))
+    return -1;
   JoinArgs a{};
   a.ctx = reinterpret_cast<const detail::Context *>(runtime::rt().driver_ctx_handle(my_pe).ctx_opaque);
   a.partial = static_cast<const char *>(partial);

@@ -304,6 +304,8 @@ void attend_kernel(AttendArgs a) {
   // pieces lie turned by r: a piece's place comes from turning what is fetched.
   const uint32_t d = a.cache.head_dim, row_bytes = a.cache.row_bytes, pieces = row_bytes / 16;
   const auto turn = [&](uint32_t row) { return pieces < 16 ? row * pieces / 16 : row; };
+  constexpr uint32_t kFewest = (kDim == 64 ? 16 : kDim / 2 + 16) * kBytes / 16;  // pieces of a row
+  const bool narrow_rows = pieces < 4 * kKeyLoads;
   uint32_t key_from[kKeyLoads], key_at[kKeyLoads];
 #pragma unroll
   for (int j = 0; j < kKeyLoads; ++j) {
@@ -311,7 +313,7 @@ void attend_kernel(AttendArgs a) {
     const uint32_t piece = p >= turn(row) ? p - turn(row) : p + pieces - turn(row);
     key_from[j] = row < 16 ? row * row_bytes + piece * 16 : 0;  // beyond the unit: its start again
     uint32_t want = 4 * j + quad;
-    if (want >= pieces) want = 0;  // beyond the row: its start again, against a zero of the query
+    if (want >= pieces) want = 0;  // beyond the row: not used
     want += turn(column);
     key_at[j] = column * row_bytes + (want < pieces ? want : want - pieces) * 16;
   }
@@ -430,7 +432,8 @@ void attend_kernel(AttendArgs a) {
     for (int j = 0; j < kKeyLoads; ++j)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const U4 raw = *(const __attribute__((address_space(3))) U4 *)(my_keys(u) + key_at[j]);  // NOLINT
+        U4 raw = *(const __attribute__((address_space(3))) U4 *)(my_keys(u) + key_at[j]);  // NOLINT
+        if (4 * j + 4 > static_cast<int>(kFewest) && narrow_rows && 4u * j + quad >= pieces) raw = U4{0, 0, 0, 0};
         if constexpr (kNarrow) {
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
@@ -469,14 +472,21 @@ void attend_kernel(AttendArgs a) {
   };
   const auto weigh = [&](int n, const Which &which, F4 (&s)[2], const unsigned (&scales)[2], Weights &weights) {
     if (a.softcap > 0.f) {
-      // cap tanh(x), x = s / cap:  tanh(x) = 1 - 2 / (e^2x + 1)
-      const float in_scale = 2.f * kLog2e / a.softcap;
+      // cap tanh(x), x = s / cap:  tanh(x) = 1 - 2 / (e^2x + 1), off by up to 2^-22.  Where
+      // that much of the cap is more than a score's other roundings, and x below 1/4, the
+      // Taylor series (the first term left out is 0.0089 x^11).
+      const float in_scale = 1.f / a.softcap;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float e = __builtin_amdgcn_exp2f(s[u][r] * in_scale);
-          s[u][r] = a.softcap * kLog2e * (1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f));
+          const float x = s[u][r] * in_scale, e = __builtin_amdgcn_exp2f(x * (2.f * kLog2e));
+          float t = 1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f);
+          if (a.softcap > 64.f) {
+            const float y = x * x;
+            if (y < 0.0625f) t = x + x * y * (-1.f / 3 + y * (2.f / 15 + y * (-17.f / 315 + y * (62.f / 2835))));
+          }
+          s[u][r] = a.softcap * kLog2e * t;
         }
     }
     if (which.cut) {

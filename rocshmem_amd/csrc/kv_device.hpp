@@ -145,6 +145,11 @@ inline bool extent(size_t n, size_t stride, size_t row_elems, size_t es, size_t 
   return *bytes <= static_cast<size_t>(INT64_MAX);
 }
 
+inline bool overlap(const void *a, size_t a_bytes, const void *b, size_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a_bytes && b_bytes && x < y + b_bytes && y < x + a_bytes;
+}
+
 // The cache a call works on, as its kernels see it.
 inline bool take_cache(const rocshmem_amd_kv_cache_t *cache, int my_pe, Layout *out) {
   if (!cache || !drv::valid_actor(my_pe) || !on_heap_device()) return false;

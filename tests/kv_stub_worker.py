@@ -82,7 +82,7 @@ def main():
                   dict(lse=d + 2), dict(table=None), dict(table=d + 2), dict(lengths=None), dict(lengths=d + 1),
                   dict(heads=0), dict(heads=7), dict(heads=-8), dict(heads=1 << 20), dict(n=-1), dict(n=70000),
                   dict(max_len=-1), dict(window=-1), dict(scale=float("inf")), dict(scale=float("nan")),
-                  dict(softcap=-1.0), dict(softcap=float("inf")), dict(softcap=float("nan")), dict(pages_from=2),
+                  dict(softcap=-1.0), dict(softcap=float("inf")), dict(softcap=float("nan")), dict(softcap=1e-38), dict(pages_from=2),
                   dict(pages_from=-1), dict(out_row=511), dict(q_row=BIG), dict(out_row=1 << 62),
                   dict(table_row=1 << 40), dict(pe=P), dict(pe=-1), dict(q=end - 64), dict(out=end - 64),
                   dict(lse=end - 8), dict(lengths=end - 4), dict(table=end - 4)]:
@@ -91,7 +91,7 @@ def main():
                   dict(partial=pages + 8), dict(partial=l.pe_ptr(pages, 2)), dict(partial=end - 1024), dict(lse_in=None),
                   dict(lse_in=d), dict(lse_in=pages + 2), dict(lse_in=end - 16), dict(rows=1 << 60), dict(dim=0),
                   dict(dim=12), dict(dim=-8), dict(out=None), dict(out=d + 1), dict(out=end - 8), dict(lse=d + 1),
-                  dict(lse=end - 8), dict(start=-1), dict(start=P), dict(size=0), dict(size=P + 1), dict(log_stride=-1),
+                  dict(lse=end - 8), dict(out=pages + 1024), dict(lse=pages + 4), dict(out=pages + 8176), dict(start=-1), dict(start=P), dict(size=0), dict(size=P + 1), dict(log_stride=-1),
                   dict(log_stride=40), dict(log_stride=1, size=3), dict(start=1, size=P), dict(pe=P), dict(pe=-1)]:
         calls.append(join(**other))
     for i, call in enumerate(calls):
