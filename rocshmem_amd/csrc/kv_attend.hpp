@@ -227,6 +227,8 @@ void attend_kernel(AttendArgs a) {
     const uint32_t index = quotient(static_cast<uint32_t>(unit), a.cache.by_page_units);
     return index < a.table_row ? static_cast<uint32_t>(a.page_table[b * a.table_row + index]) : ~0u;
   };
+  // Where PEs' slices are: asked for now, known when the lengths are.
+  const detail::HotWords slices = detail::hot_words(a.ctx);
   // A wavefront's units: runs of at most 64, one after the other, from `from` on.
   struct Runs {
     int from, size, each;  // of all wavefronts over all; of this one in a run
@@ -244,6 +246,7 @@ void attend_kernel(AttendArgs a) {
   bool known = a.window == 0;
   const Span span = span_of(a, b, blockIdx.x == 0 && split == 0 && threadIdx.x == 0);
   const int units = span.end_unit() - span.first_unit();
+  asm volatile("" ::"s"(slices.x), "s"(slices.y), "s"(slices.z));  // not asked for later
   bool whole = true;  // no other split has any
   if constexpr (!kWhole) {
     const Splits splits = splits_here(a, units);
@@ -274,8 +277,11 @@ void attend_kernel(AttendArgs a) {
       } else {
         const uint32_t pe = owner_of(a.cache, number);
         there = !a.own_pages || static_cast<int>(pe) == a.my_pe;
-        page = reinterpret_cast<uint64_t>(detail::remote_addr(a.ctx, a.cache.pages, static_cast<int>(pe)) +
-                                          page_offset(a.cache, number, pe));
+        // (detail::remote_addr)
+        const int64_t stride = static_cast<int64_t>(slices.x | static_cast<uint64_t>(slices.y) << 32);
+        const int64_t hop = stride ? (static_cast<int>(pe) - static_cast<int>(slices.z)) * stride
+                                   : detail::peer_hop(a.ctx, static_cast<int>(pe));
+        page = reinterpret_cast<uint64_t>(a.cache.pages) + hop + page_offset(a.cache, number, pe);
       }
     }
     page_lo = static_cast<unsigned>(page);
@@ -319,21 +325,24 @@ void attend_kernel(AttendArgs a) {
   }
   const uint32_t piece = column * kCols * kBytes;  // beyond the row: columns that nobody reads
   const uint32_t value_at = 4 * quad * row_bytes + (piece < row_bytes ? piece : 0);
-  typename QM::V query[kDots];
-  for (int n = kQueryInLds ? wave : 0; n < kTiles; n += kAttendWaves) {
-    const int h = n * 16 + column;
-    const char *row = a.q + (b * a.q_row + static_cast<uint64_t>(head0 + (h < heads_here ? h : 0)) * d) * 2;
+  typename QM::V query[kDots] = {};
+  const auto load_query = [&]() __attribute__((always_inline)) {
+    for (int n = kQueryInLds ? wave : 0; n < kTiles; n += kAttendWaves) {
+      const int h = n * 16 + column;
+      const char *row = a.q + (b * a.q_row + static_cast<uint64_t>(head0 + (h < heads_here ? h : 0)) * d) * 2;
 #pragma unroll
-    for (int j = 0; j < kDots; ++j) {
-      const uint32_t e = kNarrow ? (j / 2) * 64 + quad * 16 + (j % 2) * 8 : j * 32 + quad * 8;
-      typename QM::V v{};
-      if (h < heads_here && e < d) v = load_loose<typename QM::V>(row + e * 2);
-      if constexpr (kQueryInLds)
-        sh_query[n][j][lane] = __builtin_bit_cast(U4, v);
-      else
-        query[j] = v;
+      for (int j = 0; j < kDots; ++j) {
+        const uint32_t e = kNarrow ? (j / 2) * 64 + quad * 16 + (j % 2) * 8 : j * 32 + quad * 8;
+        typename QM::V v{};
+        if (h < heads_here && e < d) v = load_loose<typename QM::V>(row + e * 2);
+        if constexpr (kQueryInLds)
+          sh_query[n][j][lane] = __builtin_bit_cast(U4, v);
+        else
+          query[j] = v;
+      }
     }
-  }
+    if constexpr (kQueryInLds) __syncthreads();
+  };
 
   F4 acc[kTiles][kCols];
   float top[kTiles], sum[kTiles];
@@ -630,10 +639,10 @@ void attend_kernel(AttendArgs a) {
   };
   if constexpr (kWhole) {
     begin_steps(wave * runs.each, known);
-    if constexpr (kQueryInLds) __syncthreads();
+    load_query();  // behind the first keys and values
     take_steps();
   } else {
-    if constexpr (kQueryInLds) __syncthreads();
+    load_query();
     for (int first = runs.from; first < end; first += runs.each * kAttendWaves) {
       begin_steps(first + wave * runs.each, known && first == runs.from);
       take_steps();
