@@ -5,7 +5,6 @@ namespace rocshmem {
 namespace kv {
 
 constexpr int kMostTokens = 1 << 25;  // of a sequence
-constexpr int64_t kWantedWorkGroups = 512;  // two for each CU
 
 // Joins a sequence's splits: out = sum_i 2^(t_i - t) o_i / sum_i 2^(t_i - t) l_i over the
 // splits that have tokens, t the largest t_i.  One work-group per sequence and
@@ -84,12 +83,11 @@ struct Cut {
   Splits splits;  // of the bound
   int units, wanted, most_splits;
 };
-static Cut cut_of(int64_t work_groups_per_split, int64_t max_tokens, bool window) {
+static Cut cut_of(const Layout &c, int64_t work_groups_per_split, int64_t max_tokens, bool window) {
   // (a window may start inside a unit)
   const int units = static_cast<int>((max_tokens + 15) / 16) + (window || max_tokens == 0 ? 1 : 0);
-  if (left_whole(units, work_groups_per_split)) return Cut{Splits{units, 1, 1}, units, 1, 1};
-  const int64_t each = (kWantedWorkGroups + work_groups_per_split - 1) / work_groups_per_split;
-  const int wanted = each > 2 ? static_cast<int>(each) : 2;
+  if (left_whole(units, work_groups_per_split, c.row_bytes)) return Cut{Splits{units, 1, 1}, units, 1, 1};
+  const int wanted = wanted_splits(work_groups_per_split, static_cast<int>(c.head_dim));
   return Cut{splits_of(units, wanted), units, wanted, static_cast<int>(most_splits(units, wanted))};
 }
 static int columns_of(int group, int head_dim) {  // tiles of 16 query heads that one work-group takes
@@ -162,7 +160,7 @@ size_t rocshmem_amd_kv_attend_bytes(const rocshmem_amd_kv_cache_t *cache, int n_
   const int group = q_heads / cache->kv_heads, columns = columns_of(group, cache->head_dim);
   const int64_t tiles = (group + 16 * columns - 1) / (16 * columns);
   return part_bytes(static_cast<size_t>(n_seqs) * q_heads,
-                    cut_of(n_seqs * tiles * cache->kv_heads, max_len, true).most_splits, c.head_dim);
+                    cut_of(c, n_seqs * tiles * cache->kv_heads, max_len, true).most_splits, c.head_dim);
 }
 
 int rocshmem_amd_kv_attend(const rocshmem_amd_kv_cache_t *cache, int dtype, const void *q, size_t q_row,
@@ -200,12 +198,12 @@ int rocshmem_amd_kv_attend(const rocshmem_amd_kv_cache_t *cache, int dtype, cons
   const int columns = columns_of(a.group, cache->head_dim);
   a.tiles = (a.group + 16 * columns - 1) / (16 * columns);
   const int64_t per_split = static_cast<int64_t>(n_seqs) * cache->kv_heads * a.tiles;
-  const size_t needed = part_bytes(rows, cut_of(per_split, max_len, true).most_splits, a.cache.head_dim);
+  const size_t needed = part_bytes(rows, cut_of(a.cache, per_split, max_len, true).most_splits, a.cache.head_dim);
   if (needed && (!workspace || !aligned_to(workspace, 16) || workspace_bytes < needed ||
                  !drv::local_ok(workspace, workspace_bytes)))
     return -1;
   // (a window or none, no more splits than that)
-  const Cut cut = cut_of(per_split, window > 0 && window < max_len ? window : max_len, window > 0);
+  const Cut cut = cut_of(a.cache, per_split, window > 0 && window < max_len ? window : max_len, window > 0);
   a.bound_splits = cut.splits;
   a.bound_units = cut.units;
   a.wanted = cut.wanted;

@@ -174,12 +174,23 @@ inline int64_t most_splits(int64_t units, int64_t wanted) {
   const int64_t by_number = wanted == 2 ? 4 : 2 * wanted + 2, by_length = units / (2 * kStep) + 2;
   return by_number < by_length ? by_number : by_length;
 }
+// How many splits the longest is cut for: 512 work-groups, two for each CU; at least
+// two, and three unless work-groups are many already or large (wavefronts of 256
+// elements take all registers).  Measured, us, for two / three: 32 sequences to 8000
+// and 8 cache heads of 64 in e4m3 42.9 / 34.8, to 4000 in bf16 of 128 53.3 / 49.3, 16
+// with 24 heads of 64 28.0 / 26.0; 64 to 4096 with 8 heads of 128 95.3 / 97.6, with 4
+// of 256 in e4m3 52.6 / 57.3.
+inline int wanted_splits(int64_t work_groups, int head_dim) {
+  const int64_t each = (512 + work_groups - 1) / work_groups, least = work_groups < 512 && head_dim <= 128 ? 3 : 2;
+  return static_cast<int>(each > least ? each : least);
+}
 // Not split are sequences of at most 48 units, three steps of a wavefront, or 72 where
-// that fills half the GPU.  Measured, us, whole / split: 1 sequence of 600 tokens and 8
-// cache heads in bf16 8.7 / 11.6, of 1000 13.7 / 11.6, 8 of 1000 14.4 / 12.1, 32 of 1000
-// 17.4 / 19.7, 16 of 2000 26.0 / 20.4.
-__host__ __device__ constexpr bool left_whole(int64_t units, int64_t work_groups) {
-  return units <= (work_groups >= 128 ? 72 : 48);
+// that fills half the GPU and rows are short.  Measured, us, whole / split: 1 sequence
+// of 600 tokens and 8 cache heads in bf16 8.7 / 11.6, of 1000 13.7 / 11.6, 8 of 1000
+// 14.4 / 12.1, 32 of 1000 17.4 / 19.7, 16 of 2000 26.0 / 20.4; 24 to 1152 with rows of
+// 256 bytes 19.0 / 21.2, of 512 bytes 37.0 / 32.5.
+constexpr bool left_whole(int64_t units, int64_t work_groups, int64_t row_bytes) {
+  return units <= (work_groups >= 128 && row_bytes <= 256 ? 72 : 48);
 }
 
 }  // namespace kv

@@ -18,6 +18,8 @@ pytestmark = pytest.mark.gpu
 CUTS = [  # source, cache, cache heads, query heads each, dim, page, lengths, bound
     # the longest in splits of more than 256 units, which a work-group's wavefronts take in two runs
     ("bf16", "bf16", 1, 3, 16, 16, [9000] + [1, 17, 0] * 100, None),
+    ("bf16", "bf16", 1, 2, 32, 16, [9001] + [1, 17, 0, 5] * 150, None),
+    ("bf16", "e4m3", 1, 1, 16, 32, [14000] + [3] * 299, 14100),
     ("fp16", "e4m3", 1, 2, 32, 48, [11111] + [40] * 270, 12000),
     # more sequences than a wavefront looks at
     ("bf16", "bf16", 1, 2, 16, 16, [3, 0, 16, 33] * 260 + [9000, 1400, 770, 2], None),
