@@ -147,10 +147,16 @@ __device__ __forceinline__ Splits splits_here(const AttendArgs &a, int own) {
   const int near = a.bound_units - a.bound_units / 4;
   int most = own;
   if (a.n_seqs <= kMostLooked) {
-    for (int i = threadIdx.x & 63; i < a.n_seqs; i += 64) {
-      const Span s = span_of(a, i, false);
+    const auto look = [&](int k) {
+      const int i = static_cast<int>(threadIdx.x & 63) + 64 * k;
+      const Span s = span_of(a, i < a.n_seqs ? i : a.n_seqs - 1, false);
       const int units = s.end_unit() - s.first_unit();
       most = units > most ? units : most;
+    };
+    look(0);
+    if (a.n_seqs > 64) {
+#pragma unroll
+      for (int k = 1; k < kMostLooked / 64; ++k) look(k);  // (all on their way at once)
     }
     if (!__any(most >= near))
       for (int hop = 32; hop; hop /= 2) {

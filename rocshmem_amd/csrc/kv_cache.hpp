@@ -156,7 +156,7 @@ constexpr int kSplitWaves = 4, kWholeWaves = 8;
 // bound of 131072 took 68 us split by the bound, 18 so.  Only where it is near the
 // bound is the bound taken, whose splits' places are known beforehand (looking costs
 // such a call about 1 us).
-constexpr int kMostLooked = 1024;       // sequences
+constexpr int kMostLooked = 256;        // sequences; with more each goes by its own length
 constexpr int kStep = 2 * kSplitWaves;  // units of a step of all wavefronts
 __host__ __device__ inline Splits splits_of(int units, int wanted) {
   if (units <= 6 * kStep) return Splits{6 * kStep, 1, 2 * kStep};  // one

@@ -23,6 +23,7 @@ CUTS = [  # source, cache, cache heads, query heads each, dim, page, lengths, bo
     ("fp16", "e4m3", 1, 2, 32, 48, [11111] + [40] * 270, 12000),
     # more sequences than a wavefront looks at
     ("bf16", "bf16", 1, 2, 16, 16, [3, 0, 16, 33] * 260 + [9000, 1400, 770, 2], None),
+    ("bf16", "bf16", 1, 2, 16, 16, [3, 0, 1500, 33, 800] * 40 + [2100], 6000),
     # query heads in two to four tiles, whole and split
     ("bf16", "bf16", 1, 32, 128, 64, [601, 5], None),
     ("fp16", "fp16", 1, 48, 128, 16, [1300, 0, 33], None),
