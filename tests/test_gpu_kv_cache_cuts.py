@@ -196,6 +196,64 @@ def test_two_graphs_and_eager_calls_at_once(rt, L, dev):
             r.free()
 
 
+@pytest.mark.parametrize("src,cache", [("bf16", "bf16"), ("fp16", "e4m3")])
+def test_a_step_over_all_pes_from_one_graph(rt, L, dev, src, cache):
+    """What a step of answering does when each PE attends to its own pages: new
+    rows put, every PE's attention, the join for every PE; captured once and
+    replayed with new rows and queries while the sequences grow."""
+    from tests.test_gpu_graph_capture import hip
+    l, h = rt.l, hip()
+    heads, group, dim, page, n = 2, 3, 64, 16, 3
+    hq, row = heads * group, 2 * heads * dim
+    r = Run(rt, L, dev, src, cache, heads, group, dim, page, [900, 1, 130])
+    r.window, r.softcap, r.scale, r.out_type, r.out_row = 0, 0.0, 0.125, "fp32", hq * dim
+    r.max_len = r.table.shape[1] * page
+    most = r.lengths.copy()
+    r.lengths = np.maximum(most - 4, 0).astype(np.int32)
+    kv, slots, lengths = dev(np.zeros((n, row), np.uint16)), dev(np.zeros(n, np.int64)), dev(r.lengths)
+    q, table = dev(r.q_raw), dev(r.table)
+    r.ws_bytes = l.kv_attend_bytes(r.h.c, n, hq, r.max_len)
+    ws = [dev.blank(r.ws_bytes) for _ in range(P)]
+    partial, partial_lse = l.malloc(n * hq * dim * 4), l.malloc(n * hq * 4)
+    joined = [(dev.blank(n * hq * dim * 4), dev.blank(n * hq * 4)) for _ in range(P)]
+    stream, graph, exe = C.c_void_p(), C.c_void_p(), C.c_void_p()
+    assert h.hipStreamCreate(C.byref(stream)) == 0
+    try:
+        assert h.hipStreamBeginCapture(stream, 0) == 0
+        rc = [l.kv_put(r.h.as_of(L, 2), type_of(L, src), kv, row, kv + row, row, slots, n, 2, stream)]
+        for pe in range(P):
+            rc.append(l.kv_attend(r.h.as_of(L, pe), type_of(L, src), q, r.q_raw.shape[1] * dim, hq, L.FLOAT,
+                                  l.pe_ptr(partial, pe), hq * dim, l.pe_ptr(partial_lse, pe), table, r.table.shape[1],
+                                  lengths, n, r.max_len, 0, 0.125, 0.0, L.KV_OWN_PAGES, ws[pe], r.ws_bytes, pe, stream))
+        for pe in range(P):
+            rc.append(l.kv_join(L.FLOAT, l.pe_ptr(partial, pe), l.pe_ptr(partial_lse, pe), n * hq, dim, L.FLOAT,
+                                *joined[pe], 0, 0, P, pe, stream))
+        assert h.hipStreamEndCapture(stream, C.byref(graph)) == 0 and not any(rc)
+        assert h.hipGraphInstantiate(C.byref(exe), graph, None, None, 0) == 0
+        for _ in range(4):
+            at = r.lengths.copy()
+            r.lengths = np.minimum(at + 1, most).astype(np.int32)
+            new = np.array([int(r.table[b, i // page]) * page + i % page if i < r.lengths[b] else -1
+                            for b, i in enumerate(at)], np.int64)
+            raw, x = values(r.rng, (n, 2 * heads, dim), src, 0.3)
+            r.q_raw, r.q = values(r.rng, r.q_raw.shape, src, 0.3)
+            r.m.put(new, x[:, :heads], x[:, heads:])
+            for ptr, a in ((kv, raw), (slots, new), (lengths, r.lengths), (q, r.q_raw)):
+                rt.put_bytes(ptr, a)
+            assert h.hipGraphLaunch(exe, stream) == 0 and h.hipStreamSynchronize(stream) == 0
+            for pe in range(P):
+                r.ws, (r.out, r.lse) = ws[pe], joined[pe]
+                r.check()  # the join's roundings are far inside the bound for the sums over the tokens
+    finally:
+        if exe.value:
+            h.hipGraphExecDestroy(exe)
+            h.hipGraphDestroy(graph)
+        h.hipStreamDestroy(stream)
+        l.free(partial)
+        l.free(partial_lse)
+        r.free()
+
+
 def test_join_refuses_to_write_over_what_it_reads(rt, L, dev):
     l = rt.l
     part, lse = l.malloc(8 * 64 * 4), l.malloc(32)
@@ -285,6 +343,47 @@ def test_on_a_cached_heap(rt, L):
     finally:
         rt.down()
         os.environ.pop("ROCSHMEM_EMU_HEAP_CACHED", None)
+
+
+@pytest.mark.parametrize("npes", [1, 3])
+def test_other_numbers_of_pes(rt, L, npes):
+    rt.down()
+    l = rt.up(npes, HEAP)
+    d = Dev(rt)
+    try:
+        m = ref.Cache("e4m3", npes, 5, 16, 3, 48)
+        h = OnHeap(rt, L, m)
+        rng = np.random.default_rng(npes)
+        slots = rng.permutation(m.slots)[:m.slots - 3].astype(np.int64)
+        slots = np.append(slots, m.slots)  # the one that is not there
+        raw, x = values(rng, (len(slots), 6, 48), "fp16")
+        kv, d_slots = d(raw), d(slots)
+        l.kv_refused(1)
+        assert l.kv_put(h.as_of(L, npes - 1), L.HALF, kv, 288, kv + 288, 288, d_slots, len(slots), npes - 1, None) == 0
+        l.stream_sync(None)
+        m.put(slots, x[:, :3], x[:, 3:])
+        assert np.array_equal(h.download(), m.raw) and l.kv_refused(1) == 1
+        table = rng.permutation(5 * npes).astype(np.int32)
+        length = 5 * npes * 16 - 16
+        seen = ref.tokens_of(length, length, table, 16, 5 * npes)
+        filled = np.isin(seen, slots)
+        m.put(np.array(seen)[~filled], np.ones(((~filled).sum(), 3, 48)), np.ones(((~filled).sum(), 3, 48)))
+        h.upload()
+        q_raw, q = values(rng, (6, 48), "fp16", 0.3)
+        out, lse = d.blank(6 * 48 * 4), d.blank(24)
+        assert l.kv_attend(h.c, L.HALF, d(q_raw), 0, 6, L.FLOAT, out, 288, lse, d(table), len(table),
+                           d(np.array([length], np.int32)), 1, length, 0, 0.1, 0.0, 0, None, 0, 0, None) == 0
+        l.stream_sync(None)
+        got = d.read(out, 6 * 48 * 4).view(np.float32).reshape(6, 48).astype(np.float64)
+        k, v = (m.rows(seen, value) for value in (0, 1))
+        for i in range(6):
+            want, _, bound, _ = ref.attend(q[i], k[:, i // 2], v[:, i // 2], 0.1, 0.0)
+            assert (np.abs(got[i] - want) <= bound + ref.U["fp32"] * (np.abs(want) + bound)).all()
+        h.free()
+    finally:
+        l.stream_sync(None)
+        d.free()
+        rt.down()
 
 
 @pytest.mark.parametrize("nprocs", [2, 3])
