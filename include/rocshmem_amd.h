@@ -740,8 +740,9 @@ int rocshmem_amd_kv_get(const rocshmem_amd_kv_cache_t *cache, int dtype, void *k
  *   out = sum_i exp(s_i) v_i / sum_i exp(s_i),   lse = log sum_i exp(s_i)
  *
  * with the sums over the tokens that take part; where none does, out is 0 and
- * lse -infinity.  Scores, statistics and sums are held in 32 bits, the sums until
- * the end undivided: values beyond 2^90 in magnitude may overflow them.
+ * lse -infinity.  Scores, weights, statistics and sums are held in 32 bits
+ * (weights of an fp16 cache in 22), the sums until the end undivided: values
+ * beyond 2^90 in magnitude may overflow them.
  * pages_from: ROCSHMEM_AMD_KV_ALL_PAGES, or ROCSHMEM_AMD_KV_OWN_PAGES — only the
  * tokens whose page my_pe owns take part, and rocshmem_amd_kv_join of the PEs'
  * results is the attention over all of them.

@@ -1,0 +1,88 @@
+"""What the key-value cache's attention holds in 32 bits.  Scores are exact
+here (queries and keys with one element that is not 0), so that the tolerances
+count the roundings of one quantity at a time, each 2^-24 of it at most unless
+said otherwise."""
+import numpy as np
+import pytest
+
+from tests import kv_reference as ref
+from tests.test_gpu_kv_cache import HEAP, P, Dev, OnHeap, dev, type_of  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [("bf16", "bf16"), ("fp16", "fp16"), ("bf16", "e4m3"), ("fp16", "e4m3")]
+HALF_STEP = 2.0 ** -24
+
+
+class Given:
+    """Sequences with given keys and values, [b] -> [tokens, dim], one cache head."""
+
+    def __init__(self, rt, L, dev, src, cache, keys, values, page=16):
+        self.l, self.L, self.dev, self.src = rt.l, L, dev, src
+        dim = keys[0].shape[1]
+        need = [-(-len(k) // page) for k in keys]
+        per_pe = -(-sum(need) // P)
+        self.m = ref.Cache(cache, P, per_pe, page, 1, dim, fill=0xFF)
+        self.table = np.full((len(keys), max(need)), -1, np.int32)
+        self.lengths = np.array([len(k) for k in keys], np.int32)
+        order = np.random.default_rng(len(keys)).permutation(P * per_pe)
+        at = 0
+        for b, (k, v) in enumerate(zip(keys, values)):
+            self.table[b, :need[b]] = order[at:at + need[b]]
+            at += need[b]
+            slots = ref.tokens_of(len(k), len(k), self.table[b], page, P * per_pe)
+            self.m.put(slots, k[:, None], v[:, None])
+        self.h = OnHeap(rt, L, self.m)
+        self.dim = dim
+
+    def attend(self, q, scale=1.0, softcap=0.0, own_of=None):
+        """q: [sequences, heads, dim], values that the type holds; fp32 results."""
+        l, n, hq = self.l, len(self.lengths), q.shape[1]
+        bound = int(self.lengths.max())
+        out, lse = self.dev.blank(n * hq * self.dim * 4), self.dev.blank(n * hq * 4)
+        nbytes = l.kv_attend_bytes(self.h.c, n, hq, bound)
+        pe = own_of or 0
+        raw = ref.encode(q.astype(np.float32), self.src)
+        assert np.array_equal(ref.decode(raw, self.src), q)
+        assert l.kv_attend(self.h.as_of(self.L, pe), type_of(self.L, self.src), self.dev(raw), hq * self.dim, hq,
+                           self.L.FLOAT, out, hq * self.dim, lse, self.dev(self.table), self.table.shape[1],
+                           self.dev(self.lengths), n, bound, 0, scale, softcap, 0 if own_of is None else 1,
+                           self.dev.blank(nbytes), nbytes, pe, None) == 0
+        l.stream_sync(None)
+        return (self.dev.read(out, n * hq * self.dim * 4).view(np.float32).reshape(n, hq, self.dim).astype(np.float64),
+                self.dev.read(lse, n * hq * 4).view(np.float32).reshape(n, hq).astype(np.float64))
+
+
+def held(x, name):
+    """The nearest values that a format holds."""
+    return ref.decode(ref.encode(np.asarray(x, np.float32), name), name)
+
+
+@pytest.mark.parametrize("src,cache", TYPES)
+def test_weights_keep_32_bits(rt, L, dev, src, cache):
+    """Two tokens, one with score 0 and one with -x, values 1 in a column each:
+    out is 1 / (1 + w) and w / (1 + w) with w = exp(-x)."""
+    n, hq, dim, dim_v = 24, 32, 16, 16
+    rng = np.random.default_rng(6)
+    x = held(rng.uniform(0.01, 3.0, (n, hq)), "bf16")
+    x = held(x, src)
+    k, v = np.zeros((2, dim)), np.zeros((2, dim_v))
+    k[1, 0], v[0, 3], v[1, 5] = -1.0, 1.0, 1.0
+    g = Given(rt, L, dev, src, cache, [k] * n, [v] * n)
+    q = np.zeros((n, hq, dim))
+    q[..., 0] = x
+    out, lse = g.attend(q)
+    w = np.exp(-x)
+    # w: its argument by two roundings (log2 e, the product) of x each, the exponential 2;
+    # a weight kept as two 16-bit parts of fp16 another 4.  out: the sums over the
+    # tokens and of the weights, up to 4 additions each, a quotient (2) and a product.
+    of_w = (2 * x + 2 + (4 if cache == "fp16" else 0)) * HALF_STEP
+    bound = of_w + 11 * HALF_STEP
+    assert (np.abs(out[..., 5] / (w / (1 + w)) - 1) <= bound).all(), np.abs(out[..., 5] / (w / (1 + w)) - 1).max()
+    assert (np.abs(out[..., 3] / (1 / (1 + w)) - 1) <= bound).all()
+    # log(1 + w) <= log 2: the sum's roundings, the logarithm's 2^-22, and (fp16: weights
+    # lie 2^7 above the exponentials) a sum of at most 8
+    assert (np.abs(lse - np.log1p(w)) <= of_w + 2.0 ** -21 + (8 * 2.0 ** -23 if cache == "fp16" else 0)).all()
+    rest = np.delete(out, (3, 5), axis=-1)
+    assert (rest == 0).all()
+    g.h.free()
