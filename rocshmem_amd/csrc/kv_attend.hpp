@@ -511,7 +511,7 @@ void attend_kernel(AttendArgs a) {
             const float y = x * x;
             if (y < 0.0625f) t = x + x * y * (-1.f / 3 + y * (2.f / 15 + y * (-17.f / 315 + y * (62.f / 2835))));
           }
-          s[u][r] = a.softcap * kLog2e * t;
+          s[u][r] = a.softcap * (kLog2e * t);  // (the largest caps times log2 e would be infinite)
         }
     }
     if (which.cut) {

@@ -86,3 +86,34 @@ def test_weights_keep_32_bits(rt, L, dev, src, cache):
     rest = np.delete(out, (3, 5), axis=-1)
     assert (rest == 0).all()
     g.h.free()
+
+
+def one_token_each(rt, L, dev, src, cache):
+    """Sequences of one token whose scores are 1280 values from 2^-10 to 3008 of
+    either sign: (sequences, queries, scores, the tokens' value as it is held)."""
+    n, hq, dim = 32, 40, 16
+    s = np.exp(np.linspace(np.log(2.0 ** -10), np.log(3e3), n * hq // 2))
+    s = held(held(np.stack([s, -s]), "bf16"), src).reshape(n, hq)
+    k = np.zeros((1, dim))
+    k[0, 0] = 1.0
+    v = held(np.random.default_rng(1).standard_normal((1, dim)), "bf16")
+    v[:, 0] = 2.0
+    g = Given(rt, L, dev, src, cache, [k] * n, [v] * n)
+    q = np.zeros((n, hq, dim))
+    q[..., 0] = s
+    return g, q, s, g.m.rows(ref.tokens_of(1, 1, g.table[0], 16, 1 << 20), 1)[0, 0]
+
+
+@pytest.mark.parametrize("src,cache", TYPES)
+def test_caps_up_to_the_largest(rt, L, dev, src, cache):
+    """A cap near or at the largest 32-bit value is none."""
+    g, q, s, v = one_token_each(rt, L, dev, src, cache)
+    for cap in (2.3e38, 2.4e38, float(np.finfo(np.float32).max)):
+        cap = float(np.float32(cap))
+        out, lse = g.attend(q, softcap=cap)
+        # a few roundings, of a quotient by the cap (below the normal numbers: of 2^-149),
+        # products by it and by log2 e and ln 2; fp16 caches add and take off 7
+        bound = 16 * HALF_STEP * np.abs(s) + 2.0 ** -149 * cap + (8 * 2.0 ** -23 if cache == "fp16" else 0)
+        assert (np.abs(lse - s) <= bound).all(), cap
+        assert (np.abs(out - v) <= 4 * HALF_STEP * np.abs(v)).all(), cap
+    g.h.free()
