@@ -497,21 +497,25 @@ void attend_kernel(AttendArgs a) {
   };
   const auto weigh = [&](int n, const Which &which, F4 (&s)[2], const unsigned (&scales)[2], Weights &weights) {
     if (a.softcap > 0.f) {
-      // cap tanh(x), x = s / cap:  tanh(x) = 1 - 2 / (e^2x + 1), off by up to 2^-22.  Where
-      // that much of the cap is more than a score's other roundings, and x below 1/4, the
-      // Taylor series (the first term left out is 0.0089 x^11).
+      // cap tanh(x), x = s / cap.  Up to x = 5/8 as s times tanh(x) / x, a polynomial in
+      // x^2 (minimax, its own error 2^-27.8), so that small scores keep their bits
+      // whatever the cap; beyond, by tanh(x) = 1 - 2 / (e^2x + 1), where that is off by at
+      // most six half steps of 2^-24.  (The largest caps times log2 e would be infinite.)
       const float in_scale = 1.f / a.softcap;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float x = s[u][r] * in_scale, e = __builtin_amdgcn_exp2f(x * (2.f * kLog2e));
-          float t = 1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f);
-          if (a.softcap > 64.f) {
-            const float y = x * x;
-            if (y < 0.0625f) t = x + x * y * (-1.f / 3 + y * (2.f / 15 + y * (-17.f / 315 + y * (62.f / 2835))));
-          }
-          s[u][r] = a.softcap * (kLog2e * t);  // (the largest caps times log2 e would be infinite)
+          const float x = s[u][r] * in_scale, y = x * x;
+          float t = __builtin_fmaf(y, -0.005704987f, 0.020639088f);
+          t = __builtin_fmaf(y, t, -0.053739715f);
+          t = __builtin_fmaf(y, t, 0.13331442f);
+          t = __builtin_fmaf(y, t, -0.3333328f);
+          const float near = s[u][r] * (kLog2e * __builtin_fmaf(y, t, 1.f));
+          const float e = __builtin_amdgcn_exp2f(__builtin_fabsf(x) * (2.f * kLog2e));
+          t = __builtin_fmaf(-2.f, __builtin_amdgcn_rcpf(e + 1.f), 1.f);
+          const float far = __builtin_copysignf(a.softcap * (kLog2e * t), x);
+          s[u][r] = y < 0.390625f ? near : far;
         }
     }
     if (which.cut) {

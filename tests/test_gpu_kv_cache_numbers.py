@@ -117,3 +117,23 @@ def test_caps_up_to_the_largest(rt, L, dev, src, cache):
         assert (np.abs(lse - s) <= bound).all(), cap
         assert (np.abs(out - v) <= 4 * HALF_STEP * np.abs(v)).all(), cap
     g.h.free()
+
+
+@pytest.mark.parametrize("src,cache", TYPES)
+def test_capped_scores_keep_32_bits(rt, L, dev, src, cache):
+    g, q, s, v = one_token_each(rt, L, dev, src, cache)
+    for cap in (2.0 ** -100, 1e-3, 1.0, 20.0, 30.0, 50.0, 63.0, 65.0, 1000.0, 1e30, 2.4e38,
+                float(np.finfo(np.float32).max)):
+        cap = float(np.float32(cap))
+        out, lse = g.attend(q, softcap=cap)
+        want = cap * np.tanh(s / cap)
+        # The quotient by the cap 2, which tanh passes on by at most 0.8 of that; tanh
+        # by an exponential and a reciprocal 6, by a polynomial less; the factors log2 e,
+        # cap and ln 2 with their products 4: 12, and 16 allowed.
+        bound = 16 * HALF_STEP * np.abs(want)
+        if cache == "fp16":  # weights lie 2^7 above the exponentials: 7 is taken off and added again
+            bound = bound + 8 * 2.0 ** -23
+        off = np.abs(lse - want)
+        assert (off <= bound).all(), (cap, float((off / bound).max()), s.ravel()[(off / bound).argmax()])
+        assert (np.abs(out - v) <= 4 * HALF_STEP * np.abs(v)).all(), cap  # its only token's value
+    g.h.free()
