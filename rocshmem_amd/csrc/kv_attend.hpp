@@ -742,7 +742,8 @@ void attend_kernel(AttendArgs a) {
 #pragma unroll
       for (int w = 0; w < kAttendWaves; ++w) {
         const float t = sh_top[w][n * 16 + h];
-        total += t == -INFINITY ? 0.f : sh_sum[w][n * 16 + h] * __builtin_amdgcn_exp2f(t - from);
+        // (a sum without a maximum is 0, or NaN from NaN scores alone, which lse has to say)
+        total += sh_sum[w][n * 16 + h] * (t == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(t - from));
 #pragma unroll
         for (int y = 0; y < 8; ++y) x[y] += sh.out[w][h][e + y];
       }

@@ -1,7 +1,7 @@
-"""What the key-value cache's attention holds in 32 bits.  Scores are exact
-here (queries and keys with one element that is not 0), so that the tolerances
-count the roundings of one quantity at a time, each 2^-24 of it at most unless
-said otherwise."""
+"""What the key-value cache's attention holds in 32 bits, and a NaN on its way
+through out, lse and join.  Where tolerances are stated scores are exact (queries
+and keys with one element that is not 0), so that they count the roundings of
+one quantity at a time, each 2^-24 of it at most unless said otherwise."""
 import numpy as np
 import pytest
 
@@ -136,4 +136,42 @@ def test_capped_scores_keep_32_bits(rt, L, dev, src, cache):
         off = np.abs(lse - want)
         assert (off <= bound).all(), (cap, float((off / bound).max()), s.ravel()[(off / bound).argmax()])
         assert (np.abs(out - v) <= 4 * HALF_STEP * np.abs(v)).all(), cap  # its only token's value
+    g.h.free()
+
+
+@pytest.mark.parametrize("src,cache", TYPES)
+def test_a_nan_score_reaches_out_and_lse(rt, L, dev, src, cache):
+    """A sequence with NaN among the scores of its tokens, or with nothing else,
+    is NaN in out and in lse, so that a join does not take it for one without
+    tokens; its neighbours are not."""
+    rng, dim = np.random.default_rng(2), 32
+    lengths = [1, 1, 40, 40, 40, 900, 900, 2000, 17]
+    bad = [[0], [], range(40), [39], [], range(900), [450], [], range(17)]
+    keys = [held(rng.standard_normal((n, dim)), "bf16") for n in lengths]
+    values = [held(rng.standard_normal((n, dim)), "bf16") for n in lengths]
+    for k, at in zip(keys, bad):
+        k[list(at), 3] = np.nan
+    g = Given(rt, L, dev, src, cache, keys, values)
+    q = held(held(rng.standard_normal((len(lengths), 3, dim)), "bf16"), src)
+    spoiled = np.array([len(at) > 0 for at in bad])
+    for softcap in (0.0, 20.0):
+        out, lse = g.attend(q, scale=0.25, softcap=softcap)
+        assert np.isnan(out[spoiled]).all() and np.isnan(lse[spoiled]).all(), lse
+        assert np.isfinite(out[~spoiled]).all() and np.isfinite(lse[~spoiled]).all()
+    # each PE over its own pages, and the join of all
+    l, n = rt.l, len(lengths) * 3
+    partial, lses = l.malloc(n * dim * 4), l.malloc(n * 4)
+    for pe in range(P):
+        out, lse = g.attend(q, scale=0.25, own_of=pe)
+        rt.put_bytes(l.pe_ptr(partial, pe), out.astype(np.float32))
+        rt.put_bytes(l.pe_ptr(lses, pe), lse.astype(np.float32))
+    o, s = dev.blank(n * dim * 4), dev.blank(n * 4)
+    assert l.kv_join(L.FLOAT, partial, lses, n, dim, L.FLOAT, o, s, 0, 0, P, 0, None) == 0
+    l.stream_sync(None)
+    out = dev.read(o, n * dim * 4).view(np.float32).reshape(-1, 3, dim)
+    lse = dev.read(s, n * 4).view(np.float32).reshape(-1, 3)
+    assert np.isnan(out[spoiled]).all() and np.isnan(lse[spoiled]).all()
+    assert np.isfinite(out[~spoiled]).all() and np.isfinite(lse[~spoiled]).all()
+    l.free(partial)
+    l.free(lses)
     g.h.free()
