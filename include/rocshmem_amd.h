@@ -757,9 +757,11 @@ int rocshmem_amd_kv_get(const rocshmem_amd_kv_cache_t *cache, int dtype, void *k
  * a call finds, a generous bound costs a few us).  A length above max_len, or
  * above what table_row pages hold, counts as that (and is counted as refused);
  * a negative one as 0 (the same).
- * workspace: device memory of at least rocshmem_amd_kv_attend_bytes bytes,
- * 16-byte aligned, whose content does not matter; calls that may overlap in
- * time need one each. */
+ * workspace: device memory of at least rocshmem_amd_kv_attend_bytes bytes (0 if
+ * there is no such call), 16-byte aligned, whose content does not matter; calls
+ * that may overlap in time need one each.  What that says for n_seqs and max_len
+ * serves every call with at most as many sequences and a bound at most as large,
+ * so a batch that shrinks keeps its workspace. */
 enum rocshmem_amd_kv_pages_from { ROCSHMEM_AMD_KV_ALL_PAGES = 0, ROCSHMEM_AMD_KV_OWN_PAGES = 1 };
 size_t rocshmem_amd_kv_attend_bytes(const rocshmem_amd_kv_cache_t *cache, int n_seqs, int q_heads,
                                     int max_len);

@@ -160,8 +160,17 @@ size_t rocshmem_amd_kv_attend_bytes(const rocshmem_amd_kv_cache_t *cache, int n_
   if (n_seqs < 1 || n_seqs > 65535 || max_len < 1 || max_len > kMostTokens || q_heads < 1 || q_heads > 65535 || q_heads % cache->kv_heads) return 0;
   const int group = q_heads / cache->kv_heads, columns = columns_of(group, cache->head_dim);
   const int64_t tiles = (group + 16 * columns - 1) / (16 * columns);
-  return part_bytes(static_cast<size_t>(n_seqs) * q_heads,
-                    cut_of(c, n_seqs * tiles * cache->kv_heads, max_len, true).most_splits, c.head_dim);
+  // Fewer sequences are cut into more splits and may need more, up to as many as make
+  // kManyGroups work-groups; from there on they are all cut alike.  (Shorter sequences
+  // never have more splits than longer ones.)
+  const int64_t per_seq = tiles * cache->kv_heads;
+  size_t most = 0;
+  for (int64_t n = 1; n <= n_seqs; n = n * per_seq < kManyGroups || n == n_seqs ? n + 1 : n_seqs) {
+    const size_t bytes = part_bytes(static_cast<size_t>(n) * q_heads,
+                                    cut_of(c, n * per_seq, max_len, true).most_splits, c.head_dim);
+    if (bytes > most) most = bytes;
+  }
+  return most;
 }
 
 int rocshmem_amd_kv_attend(const rocshmem_amd_kv_cache_t *cache, int dtype, const void *q, size_t q_row,

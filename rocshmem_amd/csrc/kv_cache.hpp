@@ -174,6 +174,7 @@ inline int64_t most_splits(int64_t units, int64_t wanted) {
   const int64_t by_number = wanted == 2 ? 4 : 2 * wanted + 2, by_length = units / (2 * kStep) + 2;
   return by_number < by_length ? by_number : by_length;
 }
+constexpr int64_t kManyGroups = 512;
 // How many splits the longest is cut for: 512 work-groups, two for each CU; at least
 // two, and three unless work-groups are many already or large (wavefronts of 256
 // elements take all registers).  Measured, us, for two / three: 32 sequences to 8000
@@ -181,7 +182,8 @@ inline int64_t most_splits(int64_t units, int64_t wanted) {
 // with 24 heads of 64 28.0 / 26.0; 64 to 4096 with 8 heads of 128 95.3 / 97.6, with 4
 // of 256 in e4m3 52.6 / 57.3.
 inline int wanted_splits(int64_t work_groups, int head_dim) {
-  const int64_t each = (512 + work_groups - 1) / work_groups, least = work_groups < 512 && head_dim <= 128 ? 3 : 2;
+  const int64_t each = (kManyGroups + work_groups - 1) / work_groups;
+  const int64_t least = work_groups < kManyGroups && head_dim <= 128 ? 3 : 2;
   return static_cast<int>(each > least ? each : least);
 }
 // Not split are sequences of at most 48 units, three steps of a wavefront, or 72 where
