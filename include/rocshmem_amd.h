@@ -691,7 +691,8 @@ int rocshmem_amd_ctx_cycle(rocshmem_amd_team_t team, int n_wgs, int wg_size, int
  * a barrier (or stream order, where all PEs share the stream).  Slots, page
  * numbers and lengths are read by the kernels; what is out of range is left
  * out, never followed, and counted (rocshmem_amd_kv_refused).  What a call
- * writes overlaps nothing that it reads, nor its other outputs. */
+ * writes overlaps nothing that it reads, nor its other outputs.  They return 0,
+ * or -1 where a call is refused (nothing launched) or cannot be launched. */
 typedef struct rocshmem_amd_kv_cache {
   void *pages;      /* symmetric: pages_per_pe * page_bytes per PE, 16-byte aligned */
   int dtype;        /* ROCSHMEM_AMD_BF16, _HALF or _E4M3 */

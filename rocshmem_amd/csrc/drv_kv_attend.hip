@@ -100,50 +100,37 @@ static size_t part_bytes(size_t rows, size_t splits, size_t head_dim) {
 }
 
 template <int kQ, int kC, int kDim, int kTiles>
-static void launch_one(const AttendArgs &a, int n_seqs, hipStream_t s) {
+static bool launch_one(const AttendArgs &a, int n_seqs, hipStream_t s) {
   const dim3 grid(a.cache.kv_heads * a.tiles, n_seqs, a.most_splits);
-  if (a.most_splits == 1)
-    hipLaunchKernelGGL((attend_kernel<kQ, kC, kDim, kTiles, true>), grid, dim3(64 * kWholeWaves), 0, s, a);
-  else
-    hipLaunchKernelGGL((attend_kernel<kQ, kC, kDim, kTiles, false>), grid, dim3(64 * kSplitWaves), 0, s, a);
+  if (a.most_splits == 1) return launch(attend_kernel<kQ, kC, kDim, kTiles, true>, grid, 64 * kWholeWaves, s, a);
+  return launch(attend_kernel<kQ, kC, kDim, kTiles, false>, grid, 64 * kSplitWaves, s, a);
 }
 template <int kQ, int kC, int kDim>
-static void launch_columns(const AttendArgs &a, int n_seqs, int columns, hipStream_t s) {
+static bool launch_columns(const AttendArgs &a, int n_seqs, int columns, hipStream_t s) {
   if constexpr (kDim <= 128) {
     if (columns == 2) return launch_one<kQ, kC, kDim, 2>(a, n_seqs, s);
     if (columns == 3) return launch_one<kQ, kC, kDim, 3>(a, n_seqs, s);
     if (columns == 4) return launch_one<kQ, kC, kDim, 4>(a, n_seqs, s);
   }
-  launch_one<kQ, kC, kDim, 1>(a, n_seqs, s);
+  return launch_one<kQ, kC, kDim, 1>(a, n_seqs, s);
+}
+// A wavefront for a row where there are few splits, four otherwise.
+template <int kLanes>
+static bool launch_join(const AttendArgs &a, int n_seqs, hipStream_t s) {
+  const dim3 rows(a.q_heads, n_seqs);
+  if (a.most_splits <= 4 * 64 / kLanes) return launch(attend_join_kernel<kLanes, 64>, rows, 64, s, a);
+  return launch(attend_join_kernel<kLanes, 256>, rows, 256, s, a);
 }
 template <int kQ, int kC>
-static void launch_attend(const AttendArgs &a, int n_seqs, hipStream_t s) {
+static bool launch_attend(const AttendArgs &a, int n_seqs, hipStream_t s) {
   const int columns = columns_of(a.group, static_cast<int>(a.cache.head_dim));
-  if (a.cache.head_dim <= 64)
-    launch_columns<kQ, kC, 64>(a, n_seqs, columns, s);
-  else if (a.cache.head_dim <= 128)
-    launch_columns<kQ, kC, 128>(a, n_seqs, columns, s);
-  else
-    launch_columns<kQ, kC, 256>(a, n_seqs, columns, s);
-  DRV_CHECK_HIP(hipGetLastError());
-  if (a.most_splits > 1) {
-    // A wavefront for a row where there are few splits, four otherwise.
-    const auto join = [&](auto lanes) {
-      constexpr int kLanes = decltype(lanes)::value;
-      const dim3 rows(a.q_heads, n_seqs);
-      if (a.most_splits <= 4 * 64 / kLanes)
-        hipLaunchKernelGGL((attend_join_kernel<kLanes, 64>), rows, dim3(64), 0, s, a);
-      else
-        hipLaunchKernelGGL((attend_join_kernel<kLanes, 256>), rows, dim3(256), 0, s, a);
-    };
-    if (a.cache.head_dim <= 64)
-      join(std::integral_constant<int, 16>{});
-    else if (a.cache.head_dim <= 128)
-      join(std::integral_constant<int, 32>{});
-    else
-      join(std::integral_constant<int, 64>{});
-    DRV_CHECK_HIP(hipGetLastError());
-  }
+  const bool done = a.cache.head_dim <= 64    ? launch_columns<kQ, kC, 64>(a, n_seqs, columns, s)
+                    : a.cache.head_dim <= 128 ? launch_columns<kQ, kC, 128>(a, n_seqs, columns, s)
+                                              : launch_columns<kQ, kC, 256>(a, n_seqs, columns, s);
+  if (!done || a.most_splits == 1) return done;
+  if (a.cache.head_dim <= 64) return launch_join<16>(a, n_seqs, s);
+  if (a.cache.head_dim <= 128) return launch_join<32>(a, n_seqs, s);
+  return launch_join<64>(a, n_seqs, s);
 }
 
 }  // namespace kv
@@ -240,15 +227,16 @@ int rocshmem_amd_kv_attend(const rocshmem_amd_kv_cache_t *cache, int dtype, cons
   a.scale = scale;
   a.softcap = softcap;
   hipStream_t s = drv::as_stream(stream);
+  bool done;
   if (cache->dtype == ROCSHMEM_AMD_BF16)
-    launch_attend<ROCSHMEM_AMD_BF16, ROCSHMEM_AMD_BF16>(a, n_seqs, s);
+    done = launch_attend<ROCSHMEM_AMD_BF16, ROCSHMEM_AMD_BF16>(a, n_seqs, s);
   else if (cache->dtype == ROCSHMEM_AMD_HALF)
-    launch_attend<ROCSHMEM_AMD_HALF, ROCSHMEM_AMD_HALF>(a, n_seqs, s);
+    done = launch_attend<ROCSHMEM_AMD_HALF, ROCSHMEM_AMD_HALF>(a, n_seqs, s);
   else if (dtype == ROCSHMEM_AMD_BF16)
-    launch_attend<ROCSHMEM_AMD_BF16, ROCSHMEM_AMD_E4M3>(a, n_seqs, s);
+    done = launch_attend<ROCSHMEM_AMD_BF16, ROCSHMEM_AMD_E4M3>(a, n_seqs, s);
   else
-    launch_attend<ROCSHMEM_AMD_HALF, ROCSHMEM_AMD_E4M3>(a, n_seqs, s);
-  return 0;
+    done = launch_attend<ROCSHMEM_AMD_HALF, ROCSHMEM_AMD_E4M3>(a, n_seqs, s);
+  return done ? 0 : -1;
 }
 
 }  // extern "C"

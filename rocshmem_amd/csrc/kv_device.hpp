@@ -126,7 +126,18 @@ __device__ __forceinline__ void count_refused(unsigned long long *refused, unsig
   __hip_atomic_fetch_add(refused, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// ---- checks of the entry points -------------------------------------------------
+// ---- launches and checks of the entry points -------------------------------------------------
+
+// A launch's own status decides: an error that an earlier call of the program has
+// left behind for hipGetLastError is not this call's, and stays there.
+template <typename Args>
+inline bool launch(void (*kernel)(Args), dim3 grid, int lanes, hipStream_t s, const Args &a) {
+  void *args[] = {const_cast<Args *>(&a)};
+  if (hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, dim3(lanes), args, 0, s) == hipSuccess)
+    return true;
+  (void)hipGetLastError();
+  return false;
+}
 
 // The calls launch on the current device, which must be the one the heap is on.
 inline bool on_heap_device() {

@@ -69,8 +69,19 @@ def workspace(c):
     assert c.attend(1, 1 << 16, ws=ws, ws_bytes=need) == 0 and c.attend(1, 1 << 16, ws=ws, ws_bytes=need - 1) == -1
 
 
+def stale(c):
+    """An error of an earlier call, which nobody has fetched, is not these calls'."""
+    c.stub.hipPointerGetAttributes.argtypes = [C.c_void_p, C.c_void_p]
+    about = C.create_string_buffer(256)
+    for call in (c.put, c.get, c.attend, c.join):
+        assert c.stub.hipPointerGetAttributes(about, 8) != 0  # no device memory
+        before = c.launches()
+        assert call() == 0 and c.launches() == before + 1
+        assert c.stub.hipGetLastError() != 0 and c.stub.hipGetLastError() == 0  # still there, once
+
+
 if __name__ == "__main__":
     calls = Calls()
-    {"workspace": workspace}[sys.argv[1]](calls)
+    {"workspace": workspace, "stale": stale}[sys.argv[1]](calls)
     calls.l.finalize()
     print(sys.argv[1], "ok")

@@ -99,3 +99,7 @@ def run_under_the_stub(which):
 
 def test_kv_attend_takes_a_larger_batchs_workspace(L):
     run_under_the_stub("workspace")
+
+
+def test_an_earlier_calls_error_does_not_end_the_program(L):
+    run_under_the_stub("stale")
