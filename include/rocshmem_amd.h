@@ -742,8 +742,8 @@ int rocshmem_amd_kv_get(const rocshmem_amd_kv_cache_t *cache, int dtype, void *k
  *
  * with the sums over the tokens that take part; where none does, out is 0 and
  * lse -infinity.  Scores, weights, statistics and sums are held in 32 bits
- * (weights of an fp16 cache in 22), the sums until the end undivided: values
- * beyond 2^90 in magnitude may overflow them.  A NaN score makes its row of out
+ * (weights of an fp16 cache in 22), the sums until the end undivided: keys
+ * and values beyond 2^90 in magnitude may overflow them.  A NaN score makes its row of out
  * and its lse NaN; an infinite value makes its column of out NaN or infinite.
  * pages_from: ROCSHMEM_AMD_KV_ALL_PAGES, or ROCSHMEM_AMD_KV_OWN_PAGES — only the
  * tokens whose page my_pe owns take part, and rocshmem_amd_kv_join of the PEs'

@@ -175,6 +175,7 @@ int rocshmem_amd_kv_attend(const rocshmem_amd_kv_cache_t *cache, int dtype, cons
   if (n_seqs < 0 || n_seqs > 65535 || max_len < 0 || max_len > kMostTokens || window < 0) return -1;
   if (q_heads < 1 || q_heads % cache->kv_heads || q_heads > 65535) return -1;
   if (!__builtin_isfinite(scale) || !__builtin_isfinite(softcap) || softcap < 0.f) return -1;
+  if (!(__builtin_fabsf(scale) < 0x1p127f)) return -1;  // it is multiplied by log2 e
   if (softcap > 0.f && softcap < 0x1p-100f) return -1;  // scores are divided by it
   if (!n_seqs) return 0;
   const size_t row = static_cast<size_t>(q_heads) * a.cache.head_dim;

@@ -80,8 +80,17 @@ def stale(c):
         assert c.stub.hipGetLastError() != 0 and c.stub.hipGetLastError() == 0  # still there, once
 
 
+def scales(c):
+    """A scale whose product with log2 e has no 32 bits is refused."""
+    for scale in (2.0 ** 127, -2.0 ** 127, 2.4e38, 3.4028234663852886e38):
+        before = c.launches()
+        assert c.attend(scale=scale) == -1 and c.launches() == before, scale
+    for scale in (0.0, -1.0, 2.0 ** 126, 1.7e38, 1e-45):
+        assert c.attend(scale=scale) == 0, scale
+
+
 if __name__ == "__main__":
     calls = Calls()
-    {"workspace": workspace, "stale": stale}[sys.argv[1]](calls)
+    {"workspace": workspace, "stale": stale, "scales": scales}[sys.argv[1]](calls)
     calls.l.finalize()
     print(sys.argv[1], "ok")

@@ -103,3 +103,7 @@ def test_kv_attend_takes_a_larger_batchs_workspace(L):
 
 def test_an_earlier_calls_error_does_not_end_the_program(L):
     run_under_the_stub("stale")
+
+
+def test_scales_that_32_bits_do_not_hold_in_base_2_are_refused(L):
+    run_under_the_stub("scales")
