@@ -716,8 +716,9 @@ int rocshmem_amd_kv_row(const rocshmem_amd_kv_cache_t *cache, int npes, int64_t 
  * (BF16, HALF or FLOAT), token t's rows at k + t * k_row elements (v_row for v),
  * its heads one after the other; slots: n_tokens device integers.  A slot of -1
  * leaves its token out (padding).  Slots that are named twice in one call end
- * up with a mixture of the rows given for them; everything else is as if the
- * tokens had been put one after the other. */
+ * up with a mixture of the rows given for them (in E4M3 also one's codes with the
+ * other's scale); everything else is as if the tokens had been put one after the
+ * other. */
 int rocshmem_amd_kv_put(const rocshmem_amd_kv_cache_t *cache, int dtype, const void *k, size_t k_row,
                         const void *v, size_t v_row, const int64_t *slots, size_t n_tokens, int my_pe,
                         rocshmem_amd_stream_t stream);
@@ -742,9 +743,12 @@ int rocshmem_amd_kv_get(const rocshmem_amd_kv_cache_t *cache, int dtype, void *k
  *
  * with the sums over the tokens that take part; where none does, out is 0 and
  * lse -infinity.  Scores, weights, statistics and sums are held in 32 bits
- * (weights of an fp16 cache in 22), the sums until the end undivided: keys
- * and values beyond 2^90 in magnitude may overflow them.  A NaN score makes its row of out
- * and its lse NaN; an infinite value makes its column of out NaN or infinite.
+ * (weights of an fp16 cache in 22), the sums until the end undivided: keys and
+ * values beyond 2^90 in magnitude may overflow them.  A NaN score makes its row
+ * of out and its lse NaN; an infinite value makes its column of out NaN or
+ * infinite.  The order in which a sequence's sums are joined goes by the call's
+ * n_seqs, max_len and longest sequence, so the last bits of a result may differ
+ * between batches; the same call on the same data gives the same bits.
  * pages_from: ROCSHMEM_AMD_KV_ALL_PAGES, or ROCSHMEM_AMD_KV_OWN_PAGES — only the
  * tokens whose page my_pe owns take part, and rocshmem_amd_kv_join of the PEs'
  * results is the attention over all of them.

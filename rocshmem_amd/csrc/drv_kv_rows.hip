@@ -38,10 +38,13 @@ constexpr int kRuns = kCache == ROCSHMEM_AMD_E4M3 ? 2 : 1;
 // 2 * kv_heads (all keys, then all values) of 256 / kLanes neighbouring tokens, so that
 // the scale bytes of tokens in neighbouring slots leave in one store.  Bound by the
 // bytes moved: nothing but the row's largest magnitude is computed, across its
-// lanes.  65536 tokens of 8 heads x 128, 16-bit rows 12 KiB apart to and from e4m3:
-// put 94 us, get 73 us into and out of consecutive slots (4.3 and 5.5 TB/s), 99 and
-// 86 us scattered; two, four or eight tokens a group, all loads ahead, took 3 to 12 %
-// longer, and whole tokens a work-group instead of one head the same time.
+// lanes.  65536 tokens of 8 heads x 128, 16-bit rows to and from e4m3: put 83 us into
+// pages filled in order, 96 us into scattered slots (4.9 and 4.2 TB/s) from rows 12 KiB
+// apart, 80 and 94 us from rows that follow each other; get 80 and 97 us.  So it is the
+// slots that matter: a token's 128-byte pieces of 16 rows lie a page's run of rows apart
+// either way, but in order neighbouring tokens' lie together.  20011 tokens into a bf16
+// cache 32.6 and 34.2 us (5.0 and 4.8 TB/s).  Two, four or eight tokens a group, all loads
+// ahead, took 3 to 12 % longer, and whole tokens a work-group instead of one head the same time.
 template <int kSide, int kCache, int kLanes, bool kPut>
 __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
   constexpr int kGroups = 256 / kLanes, kEach = 8 * kRuns<kCache>;
@@ -232,7 +235,7 @@ __device__ __forceinline__ void store_values(char *p, const float (&x)[4]) {
 // A lane joins 16 bytes of a row.  kAtOnce members' pieces and lse's are on their
 // way together; with more members the largest lse is followed from one such batch
 // to the next.  Bound by the bytes read: 65536 rows of 128 fp32 from 8 PEs to bf16 in
-// 48.7 us, 5.9 TB/s; with work-groups of 256 lanes 51.9, through the caches 54.2, with
+// 49.7 us, 5.8 TB/s; with work-groups of 256 lanes 51.9, through the caches 54.2, with
 // 2048 work-groups that loop 56.0.
 template <int kIn, int kOut, int kAtOnce>
 __global__ __launch_bounds__(64) void join_kernel(JoinArgs a) {

@@ -4,8 +4,10 @@
 //
 // One pass over the tokens with a running maximum and sum.  The query heads that
 // share a cache head are the columns of matrix products, so keys and values are
-// read once for all of them, and nothing but the query, the running sums and two
-// steps of keys (in LDS) and values (in registers) is held:
+// read once for up to 64 of them (16 where rows are over 128 elements: a wavefront's
+// registers hold no more sums; the rest are other work-groups', which read the cache
+// again), and nothing but the query, the running sums and two steps of keys (in LDS)
+// and values (in registers) is held:
 //
 //   S^T (tokens x heads) = K Q^T,  O^T (dims x heads) += V^T P^T
 //
@@ -169,7 +171,7 @@ __device__ __forceinline__ Splits splits_here(const AttendArgs &a, int own) {
 __device__ __forceinline__ unsigned uniform(unsigned x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // Wavefronts a SIMD is to hold: as many as the registers allow without spilling in
-// the loop (a work-group of eight is two, whose four tiles at 128 spill 84 to 96 bytes).
+// the loop (a work-group of eight is two, whose four tiles at 128 spill 84 to 132 bytes).
 constexpr int waves_of(int dim, int tiles) {
   if (dim == 64) return tiles < 3 ? 3 : 2;
   if (dim == 128) return tiles == 1 ? 3 : tiles == 4 ? 1 : 2;
@@ -180,9 +182,10 @@ constexpr int waves_of(int dim, int tiles) {
 // to 16 * kTiles of the query heads that share it.  Its wavefronts share the
 // tokens out, take 32 at a step, and join their sums through LDS at the end.
 // Bound by the cache's bytes where they are many: 64 sequences to 4096 tokens, 8
-// query heads on each of 8 x 128 in bf16, 539 MB in 89 us, 6.1 TB/s; 2 to 131072 in
-// e4m3 68 us, 5.9 TB/s.  Three tiles of heads on one cache head reach 4.2 TB/s: two
-// wavefronts a SIMD, and their products between the loads.
+// query heads on each of 8 x 128 in bf16, 539 MB in 93.7 us, 5.8 TB/s (medians of 112
+// launches); 2 to 131072 in e4m3, 406 MB in 70.1 us, 5.8 TB/s.  Three tiles of heads on
+// one cache head, 185 MB in 47.0 us, reach 3.9 TB/s: two wavefronts a SIMD, and their
+// products between the loads; four, with one wavefront a SIMD, take 79 us a call.
 //
 // kQ: the activations' type, kC: the cache's; kDim: head_dim rounded up to 64, 128
 // or 256; kWhole: one split.

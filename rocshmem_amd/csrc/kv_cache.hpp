@@ -147,15 +147,21 @@ constexpr int kSplitWaves = 4, kWholeWaves = 8;
 // the order of their numbers, so the short splits fill the gaps at the end, where a
 // CU with one long split more than the others would be waited for (a CU takes little
 // more than its share of the memory's rate, so a split too many on it is not made
-// up for).  Measured, us, in equal splits / with a half in thirds: 64 sequences to
-// 4096 tokens in bf16 93.9 / 90.0, 48 heads on one 52.4 / 45.3, 16 sequences with own
-// heads 27.3 / 25.8, 2 to 131072 in e4m3 69.2 / 68.8.
+// up for).  Measured, us a call, in equal splits / with a half in thirds: 64 sequences to
+// 4096 tokens in bf16 99.5 / 95.9, 48 heads on one 56.9 / 50.4, 16 sequences with own
+// heads 29.1 / 25.9, 2 to 131072 in e4m3 74.5 / 74.9.
 //
 // The longest is the longest of the call as a wavefront finds it, not the bound that
-// a captured call has to give: 64 sequences of 400 tokens and 8 cache heads under a
-// bound of 131072 took 68 us split by the bound, 18 so.  Only where it is near the
-// bound is the bound taken, whose splits' places are known beforehand (looking costs
-// such a call about 1 us).
+// a captured call has to give.  Measured, us, split by a bound of 131072 / by the longest,
+// 8 cache heads of 128 in bf16: 1 sequence of 2000 tokens 24.8 / 14.2, 4 of 2000 37.5 /
+// 16.1, 4 of 8000 79.4 / 29.7, 16 of 2000 40.0 / 31.4; 64 of 2000, which the bound
+// leaves in one piece each, 88.6 / 96.2.  Only where it is near the bound is the bound
+// taken, whose splits' places are known beforehand (looking costs such a call about 1 us).
+//
+// How fine that is goes by the number of sequences, not by how their lengths are spread:
+// with 64 or more on 8 cache heads half of the longest is one work-group's.  Where one is
+// far longer than all others the call waits for that: 585 us for one sequence of 131072
+// tokens among 63 of 300, which take 100 and 23 us in calls of their own.
 constexpr int kMostLooked = 256;        // sequences; with more each goes by its own length
 constexpr int kStep = 2 * kSplitWaves;  // units of a step of all wavefronts
 __host__ __device__ inline Splits splits_of(int units, int wanted) {
@@ -178,19 +184,21 @@ constexpr int64_t kManyGroups = 512;
 // How many splits the longest is cut for: 512 work-groups, two for each CU; at least
 // two, and three unless work-groups are many already or large (wavefronts of 256
 // elements take all registers).  Measured, us, for two / three: 32 sequences to 8000
-// and 8 cache heads of 64 in e4m3 42.9 / 34.8, to 4000 in bf16 of 128 53.3 / 49.3, 16
-// with 24 heads of 64 28.0 / 26.0; 64 to 4096 with 8 heads of 128 95.3 / 97.6, with 4
-// of 256 in e4m3 52.6 / 57.3.
+// and 8 cache heads of 64 in e4m3 46.4 / 39.6, to 4000 in bf16 of 128 56.4 / 52.2, 16
+// with 24 heads of 64 28.3 / 26.2; 64 to 4096 with 8 heads of 128 95.9 / 98.6, with 4
+// of 256 in e4m3 57.7 / 60.9.
 inline int wanted_splits(int64_t work_groups, int head_dim) {
   const int64_t each = (kManyGroups + work_groups - 1) / work_groups;
   const int64_t least = work_groups < kManyGroups && head_dim <= 128 ? 3 : 2;
   return static_cast<int>(each > least ? each : least);
 }
 // Not split are sequences of at most 48 units, three steps of a wavefront, or 72 where
-// that fills half the GPU and rows are short.  Measured, us, whole / split: 1 sequence
-// of 600 tokens and 8 cache heads in bf16 8.7 / 11.6, of 1000 13.7 / 11.6, 8 of 1000
-// 14.4 / 12.1, 32 of 1000 17.4 / 19.7, 16 of 2000 26.0 / 20.4; 24 to 1152 with rows of
-// 256 bytes 19.0 / 21.2, of 512 bytes 37.0 / 32.5.
+// that fills half the GPU and rows are short.  Measured, us, whole / split, all sequences
+// of 1152 tokens, 72 units: rows of 256 bytes (bf16) on 64 work-groups 17.4 / 15.8, 96
+// 17.6 / 18.1, 128 18.4 / 20.4, 192 21.9 / 26.1; (e4m3) 64 20.4 / 17.8, 96 21.1 / 21.4,
+// 128 21.4 / 23.6, 192 24.0 / 33.0; of 128 bytes 64 14.3 / 13.4, 128 14.6 / 15.3, 192
+// 15.2 / 18.8; of 512 bytes 64 36.9 / 25.5, 128 39.2 / 35.3, and from 160 on 41.1 / 47.0
+// (not used).  At 900 tokens, 57 units, the order is the same.
 constexpr bool left_whole(int64_t units, int64_t work_groups, int64_t row_bytes) {
   return units <= (work_groups >= 128 && row_bytes <= 256 ? 72 : 48);
 }
